@@ -314,6 +314,34 @@ int32_t asc_cuda_gemm_i8(const int8_t* A, const int8_t* B, int32_t* acc, void* d
 int32_t asc_cuda_attn_fwd_f16(const void* q, const void* k, const void* v, void* o, int32_t B, int32_t H,
                               int32_t S, int32_t D, float scale, int32_t causal, int32_t dtype, void* stream);
 
+/* Rotary positions of queries q [B, S, Hq, D] and keys k [B, S, Hk, D] in one pass, with an RMS norm of every head in
+ * front of the rotation when flags has bit 1:
+ *   n = x / sqrt(mean_D(x^2) + eps) * gamma        (gamma: D values, NULL: ones; without bit 1: n = x)
+ *   a_i = position * frequencies[i],  i < r / 2    (a full product, so that far positions keep their angle)
+ *   lo' = scale * (lo cos a_i - hi sin a_i),  hi' = scale * (hi cos a_i + lo sin a_i);  elements from r on are n itself
+ * flags: bit 0 pairs (lo, hi) are elements (2 i, 2 i + 1), otherwise (i, i + r / 2); bit 1 norm; bit 2 positions are
+ * int32, otherwise int64; bit 3 turn back (sin negated): the gradient of the rotation without a norm.
+ * dims = {B, S, Hq, Hk, D, r}: r <= D even, D <= 1024, B * S <= 2^30; Hk or Hq may be 0 (that tensor is not touched).
+ * strides, in elements, the last dimension contiguous: q, k, q_out, k_out (three each: batch, sequence, head), then
+ * positions (batch, sequence; 0 repeats); an output stride of 0 over several elements is status 1.  dims and strides
+ * are host arrays.  dtype: 0 fp16, 1 bf16, 2 fp32 of q, k and the outputs; gamma_dtype the same for the gammas.  fp32
+ * arithmetic, one rounding at the store.  An output may be its input (same pointer and strides).  Pointers need their
+ * element's alignment; operands whose pointers and strides are multiples of 16 bytes, with D (and r / 2 for halves) a
+ * multiple of 16 bytes too, take the vector kernels.  No counterpart in the reference. */
+int32_t asc_cuda_norm_rotary(const void* q, const void* k, void* q_out, void* k_out, const void* q_gamma,
+                             const void* k_gamma, const void* positions, const double* frequencies,
+                             const int64_t* dims, const int64_t* strides, float eps, float scale, int32_t dtype,
+                             int32_t gamma_dtype, int32_t flags, void* stream);
+/* The gradients of asc_cuda_norm_rotary with norm: dq, dk (of q and k) and dq_gamma, dk_gamma (fp32, D values each,
+ * overwritten; NULL: not wanted) from the gradients dq_out, dk_out of its outputs and its inputs.  strides: dq_out,
+ * dk_out, q, k, dq, dk, positions.  flags must have bit 1 and not bit 3.  dq may be dq_out or q, dk likewise.  The sums
+ * over rows are taken in a fixed order; their workspace is allocated and released on the stream. */
+int32_t asc_cuda_norm_rotary_bwd(const void* dq_out, const void* dk_out, const void* q, const void* k, void* dq, void* dk,
+                                 const void* q_gamma, const void* k_gamma, float* dq_gamma, float* dk_gamma,
+                                 const void* positions, const double* frequencies, const int64_t* dims,
+                                 const int64_t* strides, float eps, float scale, int32_t dtype, int32_t gamma_dtype,
+                                 int32_t flags, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

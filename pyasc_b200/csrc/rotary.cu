@@ -1,0 +1,783 @@
+// Rotary positions of queries and keys, with or without an RMS norm of every head in front, and the gradients.
+//
+//   n = x * rsqrt(mean(x^2) + eps) * gamma                      (norm; otherwise n = x)
+//   a_i = position * frequency_i,  c_i = scale * cos(a_i),  s_i = scale * sin(a_i),   i < r / 2
+//   y_lo = n_lo c - n_hi s,  y_hi = n_hi c + n_lo s             over the r / 2 pairs (lo, hi) of a head: (i, i + r / 2)
+//                                                               or (2 i, 2 i + 1); elements from r on are n itself
+// Backward: dn = R^T dy, t = gamma dn, dx = rstd t - x rstd^3 mean(x t), dgamma = sum over rows of x rstd dn.
+//
+// HBM-bound: a row is read once and written once (backward: x and dy read, dx written); positions, frequencies and
+// gammas are a few hundred bytes per token or less.  Queries and keys of a token share its angles, so one launch does
+// both.  The angle is multiplied and reduced to a fraction of a turn in 64 bits and their rests: at position 10^6 a
+// 32-bit product is off by up to 0.03 rad, while sin and cos of the fraction are right in fp32.  A CTA computes the sines of its tokens into shared
+// memory once; a group of 4 to 32 lanes then owns a row and keeps both halves of each pair in one lane, so that the
+// rotation needs no exchange and the norm one shuffle reduction.  All arithmetic is fp32, one rounding at the store.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "../../include/asc_cuda.h"
+#include "host_common.h"
+
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kWarps = kThreads / 32;
+constexpr int kMaxHeadDim = 1024;
+
+struct Operand {           // a [batch, sequence, head, dim] tensor: strides in elements, dim contiguous
+  void* p;
+  int64_t b, s, h;
+};
+
+struct RotaryArgs {
+  Operand x[2], y[2];      // queries, keys: input and output (forward); x and dx (backward)
+  Operand dy[2];           // backward only
+  const void* gamma[2];    // null: ones
+  float* partial;          // backward: [CTAs, D] partial sums of dgamma
+  const void* positions;
+  const double* freq;
+  int64_t pos_b, pos_s;
+  int32_t S, tokens;       // tokens = batch * S
+  int32_t heads[2];
+  int32_t D, r;
+  int32_t log_lanes;       // lanes per row (vector kernels)
+  int32_t log_tokens;      // tokens a CTA works on at a time
+  int32_t q_ctas;          // backward: CTAs [0, q_ctas) own queries, the others keys
+  int32_t gamma_type;      // 0 fp16, 1 bf16, 2 fp32
+  int32_t pos32;           // positions are int32 instead of int64
+  int32_t norm, interleaved, conj;
+  float eps, scale;
+};
+
+__device__ __forceinline__ float to_float(float v) { return v; }
+__device__ __forceinline__ float to_float(__half v) { return __half2float(v); }
+__device__ __forceinline__ float to_float(__nv_bfloat16 v) { return __bfloat162float(v); }
+template <typename T>
+__device__ __forceinline__ T from_float(float v);
+template <>
+__device__ __forceinline__ float from_float<float>(float v) { return v; }
+template <>
+__device__ __forceinline__ __half from_float<__half>(float v) { return __float2half_rn(v); }
+template <>
+__device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+
+// 16 bytes of a row <-> fp32 registers
+template <typename T>
+struct Vec;
+template <>
+struct Vec<float> {
+  static constexpr int E = 4;
+  __device__ static void unpack(const uint4& t, float* v) {
+    v[0] = __uint_as_float(t.x), v[1] = __uint_as_float(t.y), v[2] = __uint_as_float(t.z), v[3] = __uint_as_float(t.w);
+  }
+  __device__ static uint4 pack(const float* v) {
+    return make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
+  }
+};
+template <>
+struct Vec<__half> {
+  static constexpr int E = 8;
+  __device__ static void unpack(const uint4& t, float* v) {
+    const uint32_t w[4] = {t.x, t.y, t.z, t.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+      v[2 * i] = f.x, v[2 * i + 1] = f.y;
+    }
+  }
+  __device__ static uint4 pack(const float* v) {
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const __half2 h = __floats2half2_rn(v[2 * i], v[2 * i + 1]);
+      w[i] = *reinterpret_cast<const uint32_t*>(&h);
+    }
+    return make_uint4(w[0], w[1], w[2], w[3]);
+  }
+};
+template <>
+struct Vec<__nv_bfloat16> {
+  static constexpr int E = 8;
+  __device__ static void unpack(const uint4& t, float* v) {
+    const uint32_t w[4] = {t.x, t.y, t.z, t.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      v[2 * i] = __uint_as_float(w[i] << 16), v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+  }
+  __device__ static uint4 pack(const float* v) {
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const __nv_bfloat162 h = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
+      w[i] = *reinterpret_cast<const uint32_t*>(&h);
+    }
+    return make_uint4(w[0], w[1], w[2], w[3]);
+  }
+};
+
+__device__ __forceinline__ float load_gamma(const RotaryArgs& a, int which, int i) {
+  const void* g = a.gamma[which];
+  if (g == nullptr) return 1.f;
+  if (a.gamma_type == 0) return __half2float(static_cast<const __half*>(g)[i]);
+  if (a.gamma_type == 1) return __bfloat162float(static_cast<const __nv_bfloat16*>(g)[i]);
+  return static_cast<const float*>(g)[i];
+}
+
+// scale * (cos, sin) of the angle of `token`'s pair `f`; `conj` turns back
+__device__ __forceinline__ float2 turn_of(const RotaryArgs& a, int token, int f) {
+  const int b = token / a.S, s = token - b * a.S;
+  const int64_t at = b * a.pos_b + s * a.pos_s;
+  const double pos = a.pos32 ? static_cast<double>(static_cast<const int32_t*>(a.positions)[at])
+                             : static_cast<double>(static_cast<const int64_t*>(a.positions)[at]);
+  // turns = pos * f / (2 pi) as a rounded value and what the roundings left out, so that the fraction of a turn is
+  // right to 2^-50 at any position (in plain 64 bits it would be off by 2^-16 of a turn at position 2^40)
+  constexpr double kInv2Pi = 0.15915494309189535, kInv2PiRest = -9.839338337591243e-18;
+  const double angle = pos * a.freq[f], angle_rest = fma(pos, a.freq[f], -angle);
+  const double turns = angle * kInv2Pi;
+  const double rest = fma(angle, kInv2Pi, -turns) + (angle * kInv2PiRest + angle_rest * kInv2Pi);
+  float sn, cs;
+  sincospif(static_cast<float>(2.0 * ((turns - rint(turns)) + rest)), &sn, &cs);
+  return make_float2(cs * a.scale, (a.conj ? -sn : sn) * a.scale);
+}
+
+template <typename T>
+__device__ __forceinline__ T* row_of(const Operand& o, int b, int s, int h) {
+  return static_cast<T*>(o.p) + b * o.b + s * o.s + h * o.h;
+}
+
+// Which two 16-byte vectors of a row a lane owns.  Half layout: lane < r / 2 / E owns the vectors of both halves of its
+// pairs; later lanes own two neighbours of the part that is not turned.  Interleaved: both halves of a pair lie in one
+// vector, and a lane owns vectors `lane` and `lane + ceil(n / 2)`.
+template <int E>
+struct LaneVectors {
+  int v0, v1;
+  bool has0, has1, turns;     // turns: half layout, this lane holds pairs
+  __device__ LaneVectors(const RotaryArgs& a, int lane) {
+    const int n = a.D / E;
+    if (a.interleaved) {
+      const int half = (n + 1) / 2;
+      v0 = lane, v1 = lane + half;
+      has0 = lane < half, has1 = has0 && v1 < n, turns = false;
+    } else {
+      const int hv = a.r / 2 / E;
+      turns = lane < hv;
+      v0 = turns ? lane : 2 * lane;             // 2 hv + 2 (lane - hv)
+      v1 = turns ? lane + hv : v0 + 1;
+      has0 = v0 < n, has1 = v1 < n;
+      if (turns) has0 = has1 = true;
+    }
+  }
+};
+
+// cos / sin of the pairs a lane owns, as fp32 registers.  Interleaved: the first E / 2 belong to vector v0.
+template <int E>
+__device__ __forceinline__ void lane_turns(const RotaryArgs& a, const LaneVectors<E>& l, const float2* table, float* c,
+                                           float* s) {
+  const int half_r = a.r / 2;
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    int f;
+    if (a.interleaved)
+      f = (e < E / 2 ? l.v0 : l.v1) * (E / 2) + (e & (E / 2 - 1));
+    else
+      f = l.turns ? l.v0 * E + e : half_r;
+    const float2 t = f < half_r ? table[f] : make_float2(1.f, 0.f);
+    c[e] = t.x, s[e] = t.y;
+  }
+}
+
+// Rotates the 2 E values of a lane in place.  Values that are not part of a pair are left alone, also non-finite ones.
+template <int E, bool kInter>
+__device__ __forceinline__ void rotate(const RotaryArgs& a, const LaneVectors<E>& l, const float* c, const float* s,
+                                       float* v, bool back) {
+  if (kInter) {
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      const int at = (e < E / 2 ? l.v0 : l.v1) * E + 2 * (e & (E / 2 - 1));
+      const float x = v[2 * e], y = v[2 * e + 1], sn = back ? -s[e] : s[e];
+      if (at < a.r) {
+        v[2 * e] = x * c[e] - y * sn;
+        v[2 * e + 1] = y * c[e] + x * sn;
+      }
+    }
+  } else if (l.turns) {
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      const float x = v[e], y = v[E + e], sn = back ? -s[e] : s[e];
+      v[e] = x * c[e] - y * sn;
+      v[E + e] = y * c[e] + x * sn;
+    }
+  }
+}
+
+__device__ __forceinline__ float group_sum(float v, int log_lanes) {
+  for (int o = 1 << log_lanes >> 1; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+
+// --------------------------------------------------------------------------------------------------------------
+// Forward, whole 16-byte vectors.  A CTA works on 2^log_tokens tokens; the groups of a token share its heads, queries
+// first and then keys.  The next row is loaded before the current one is computed.
+// --------------------------------------------------------------------------------------------------------------
+template <typename T, bool kNorm, bool kInter>
+__global__ void __launch_bounds__(kThreads) rotary_fwd_kernel(const RotaryArgs a) {
+  constexpr int E = Vec<T>::E;
+  extern __shared__ float2 table[];              // [tokens of this CTA][r / 2]
+  const int half_r = a.r / 2;
+  const int lane = threadIdx.x & ((1 << a.log_lanes) - 1), group = threadIdx.x >> a.log_lanes;
+  const int groups = kThreads >> a.log_lanes;
+  const int per_token = groups >> a.log_tokens;                 // groups that share a token
+  const int local = group / per_token;
+  const int token0 = blockIdx.x << a.log_tokens;
+  const int token = token0 + local;
+  const int H = a.heads[0] + a.heads[1];
+  const int step = per_token * gridDim.y;
+  const int first = blockIdx.y * per_token + (group - local * per_token);
+  const int iters = (H + step - 1) / step;
+  const LaneVectors<E> l(a, lane);
+  const int b = token / a.S, s = token - b * a.S;
+  const bool here = token < a.tokens;
+
+  auto load = [&](int h, uint4& lo, uint4& hi) {
+    lo = hi = make_uint4(0, 0, 0, 0);
+    if (!here || h >= H) return;
+    const int w = h >= a.heads[0];
+    const uint4* row = reinterpret_cast<const uint4*>(row_of<const T>(a.x[w], b, s, h - (w ? a.heads[0] : 0)));
+    if (l.has0) lo = row[l.v0];
+    if (l.has1) hi = row[l.v1];
+  };
+  uint4 lo, hi;
+  load(first, lo, hi);
+
+  const int n_angles = min(1 << a.log_tokens, a.tokens - token0) * half_r;
+  for (int i = threadIdx.x; i < n_angles; i += kThreads) {
+    const int t = i / half_r;
+    table[i] = turn_of(a, token0 + t, i - t * half_r);
+  }
+  __syncthreads();
+  float c[E], sn[E];
+  if (here) lane_turns<E>(a, l, table + local * half_r, c, sn);
+
+  float g[2 * E];
+  int which = -1;
+  const float inv_d = 1.f / a.D;
+  for (int it = 0; it < iters; ++it) {
+    const int h = first + it * step;
+    const int w = h >= a.heads[0];
+    uint4 next_lo, next_hi;
+    load(h + step, next_lo, next_hi);
+    float v[2 * E];
+    Vec<T>::unpack(lo, v);
+    Vec<T>::unpack(hi, v + E);
+    if (kNorm) {
+      if (w != which) {
+        which = w;
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+          g[e] = l.has0 ? load_gamma(a, w, l.v0 * E + e) : 0.f;
+          g[E + e] = l.has1 ? load_gamma(a, w, l.v1 * E + e) : 0.f;
+        }
+      }
+      float ss = 0.f;
+#pragma unroll
+      for (int e = 0; e < 2 * E; ++e) ss = fmaf(v[e], v[e], ss);
+      const float rstd = 1.f / sqrtf(group_sum(ss, a.log_lanes) * inv_d + a.eps);
+#pragma unroll
+      for (int e = 0; e < 2 * E; ++e) v[e] = v[e] * rstd * g[e];
+    }
+    if (here && h < H) {
+      rotate<E, kInter>(a, l, c, sn, v, false);
+      uint4* row = reinterpret_cast<uint4*>(row_of<T>(a.y[w], b, s, h - (w ? a.heads[0] : 0)));
+      if (l.has0) row[l.v0] = Vec<T>::pack(v);
+      if (l.has1) row[l.v1] = Vec<T>::pack(v + E);
+    }
+    lo = next_lo, hi = next_hi;
+  }
+}
+
+// --------------------------------------------------------------------------------------------------------------
+// Backward through norm and rotation, whole 16-byte vectors.  Each CTA owns queries or keys (so that one set of dgamma
+// sums stays in registers) and strides over the token chunks.
+// --------------------------------------------------------------------------------------------------------------
+template <typename T, bool kInter>
+__global__ void __launch_bounds__(kThreads) rotary_bwd_kernel(const RotaryArgs a) {
+  constexpr int E = Vec<T>::E;
+  extern __shared__ float2 table[];
+  __shared__ float sums[kThreads * 2 * E];       // [group][lane][2 E]
+  const int half_r = a.r / 2;
+  const int lane = threadIdx.x & ((1 << a.log_lanes) - 1), group = threadIdx.x >> a.log_lanes;
+  const int groups = kThreads >> a.log_lanes;
+  const int per_token = groups >> a.log_tokens;
+  const int local = group / per_token;
+  const int w = blockIdx.x >= a.q_ctas;
+  const int cta = w ? blockIdx.x - a.q_ctas : blockIdx.x;
+  const int ctas = w ? gridDim.x - a.q_ctas : a.q_ctas;
+  const int H = a.heads[w];
+  const int first = group - local * per_token;
+  const int iters = (H + per_token - 1) / per_token;
+  const int chunks = (a.tokens + (1 << a.log_tokens) - 1) >> a.log_tokens;
+  const LaneVectors<E> l(a, lane);
+  const Operand X = a.x[w], DY = a.dy[w], DX = a.y[w];
+  const float inv_d = 1.f / a.D;
+
+  float g[2 * E], dg[2 * E];
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    g[e] = l.has0 ? load_gamma(a, w, l.v0 * E + e) : 0.f;
+    g[E + e] = l.has1 ? load_gamma(a, w, l.v1 * E + e) : 0.f;
+    dg[e] = dg[E + e] = 0.f;
+  }
+  for (int chunk = cta; chunk < chunks; chunk += ctas) {
+    const int token0 = chunk << a.log_tokens;
+    const int token = token0 + local;
+    const bool here = token < a.tokens;
+    const int b = token / a.S, s = token - b * a.S;
+    auto load = [&](int h, uint4 (&x)[2], uint4 (&y)[2]) {
+      x[0] = x[1] = y[0] = y[1] = make_uint4(0, 0, 0, 0);
+      if (!here || h >= H) return;
+      const uint4* xr = reinterpret_cast<const uint4*>(row_of<const T>(X, b, s, h));
+      const uint4* yr = reinterpret_cast<const uint4*>(row_of<const T>(DY, b, s, h));
+      if (l.has0) x[0] = xr[l.v0], y[0] = yr[l.v0];
+      if (l.has1) x[1] = xr[l.v1], y[1] = yr[l.v1];
+    };
+    uint4 x[2], y[2];
+    load(first, x, y);
+    __syncthreads();                             // the previous chunk's angles are no longer read
+    const int n_angles = min(1 << a.log_tokens, a.tokens - token0) * half_r;
+    for (int i = threadIdx.x; i < n_angles; i += kThreads) {
+      const int t = i / half_r;
+      table[i] = turn_of(a, token0 + t, i - t * half_r);
+    }
+    __syncthreads();
+    float c[E], sn[E];
+    if (here) lane_turns<E>(a, l, table + local * half_r, c, sn);
+    for (int it = 0; it < iters; ++it) {
+      const int h = first + it * per_token;
+      const bool on = here && h < H;
+      float v[2 * E], d[2 * E];
+      Vec<T>::unpack(x[0], v);
+      Vec<T>::unpack(x[1], v + E);
+      Vec<T>::unpack(y[0], d);
+      Vec<T>::unpack(y[1], d + E);
+      load(h + per_token, x, y);
+      if (on) rotate<E, kInter>(a, l, c, sn, d, true);
+      float ss = 0.f, xt = 0.f;
+#pragma unroll
+      for (int e = 0; e < 2 * E; ++e) {
+        ss = fmaf(v[e], v[e], ss);
+        xt = fmaf(v[e] * g[e], d[e], xt);
+      }
+      ss = group_sum(ss, a.log_lanes);
+      xt = group_sum(xt, a.log_lanes);
+      const float rstd = 1.f / sqrtf(ss * inv_d + a.eps);
+      const float k = rstd * rstd * rstd * xt * inv_d;
+      if (on) {
+#pragma unroll
+        for (int e = 0; e < 2 * E; ++e) {
+          dg[e] = fmaf(v[e] * rstd, d[e], dg[e]);
+          d[e] = rstd * (g[e] * d[e]) - v[e] * k;
+        }
+        uint4* row = reinterpret_cast<uint4*>(row_of<T>(DX, b, s, h));
+        if (l.has0) row[l.v0] = Vec<T>::pack(d);
+        if (l.has1) row[l.v1] = Vec<T>::pack(d + E);
+      }
+    }
+  }
+  if (a.partial == nullptr) return;
+  // sums of this CTA in group order, then one row of partial sums per CTA: the same order in every run
+#pragma unroll
+  for (int e = 0; e < 2 * E; ++e) sums[threadIdx.x * 2 * E + e] = dg[e];
+  __syncthreads();
+  if (group == 0) {
+#pragma unroll
+    for (int e = 0; e < 2 * E; ++e) {
+      float t = 0.f;
+      for (int k = 0; k < groups; ++k) t += sums[((k << a.log_lanes) + lane) * 2 * E + e];
+      const int v = e < E ? l.v0 : l.v1;
+      if (e < E ? l.has0 : l.has1) a.partial[static_cast<int64_t>(blockIdx.x) * a.D + v * E + (e & (E - 1))] = t;
+    }
+  }
+}
+
+// --------------------------------------------------------------------------------------------------------------
+// Any head size up to 1024, any alignment: a warp owns a row and reads it twice, element by element.
+// --------------------------------------------------------------------------------------------------------------
+template <typename T, bool kBwd>
+__global__ void __launch_bounds__(kThreads) rotary_any_kernel(const RotaryArgs a) {
+  extern __shared__ float2 table[];              // r / 2 angles, then (backward) D sums for each warp
+  const int half_r = a.r / 2;
+  float* dg = reinterpret_cast<float*>(table + half_r) + (threadIdx.x >> 5) * a.D;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int w0 = kBwd && blockIdx.x >= a.q_ctas;
+  const int cta = w0 ? blockIdx.x - a.q_ctas : blockIdx.x;
+  const int ctas = !kBwd ? gridDim.x : w0 ? gridDim.x - a.q_ctas : a.q_ctas;
+  const int H = kBwd ? a.heads[w0] : a.heads[0] + a.heads[1];
+  const float inv_d = 1.f / a.D;
+  if (kBwd)
+    for (int i = lane; i < a.D; i += 32) dg[i] = 0.f;
+  for (int token = cta; token < a.tokens; token += ctas) {
+    __syncthreads();
+    for (int i = threadIdx.x; i < half_r; i += kThreads) table[i] = turn_of(a, token, i);
+    __syncthreads();
+    const int b = token / a.S, s = token - b * a.S;
+    for (int hh = warp; hh < H; hh += kWarps) {
+      const int w = kBwd ? w0 : hh >= a.heads[0];
+      const int h = !kBwd && w ? hh - a.heads[0] : hh;
+      const T* x = row_of<const T>(a.x[w], b, s, h);
+      const T* dy = kBwd ? row_of<const T>(a.dy[w], b, s, h) : nullptr;
+      T* y = row_of<T>(a.y[w], b, s, h);
+      // element p of the part that is turned pairs with element q; d = R^T dy of both
+      auto pair_at = [&](int i, int& p, int& q) {
+        p = a.interleaved ? 2 * i : i;
+        q = a.interleaved ? 2 * i + 1 : i + half_r;
+      };
+      auto turned_back = [&](int i, int p, int q, float& dp, float& dq) {
+        const float u = to_float(dy[p]), v = to_float(dy[q]);
+        dp = u * table[i].x + v * table[i].y;
+        dq = v * table[i].x - u * table[i].y;
+      };
+      float rstd = 1.f, k = 0.f;
+      if (a.norm) {
+        float ss = 0.f, xt = 0.f;
+        for (int i = lane; i < a.D; i += 32) {
+          const float t = to_float(x[i]);
+          ss = fmaf(t, t, ss);
+          if (kBwd && i >= a.r) xt = fmaf(t * load_gamma(a, w, i), to_float(dy[i]), xt);
+        }
+        if (kBwd) {
+          for (int i = lane; i < half_r; i += 32) {
+            int p, q;
+            float dp, dq;
+            pair_at(i, p, q);
+            turned_back(i, p, q, dp, dq);
+            xt = fmaf(to_float(x[p]) * load_gamma(a, w, p), dp, xt);
+            xt = fmaf(to_float(x[q]) * load_gamma(a, w, q), dq, xt);
+          }
+          xt = group_sum(xt, 5);
+        }
+        rstd = 1.f / sqrtf(group_sum(ss, 5) * inv_d + a.eps);
+        k = rstd * rstd * rstd * xt * inv_d;
+      }
+      __syncwarp();
+      if (kBwd) {
+        auto finish = [&](int i, float d) {
+          const float t = to_float(x[i]);
+          dg[i] = fmaf(t * rstd, d, dg[i]);
+          return rstd * (load_gamma(a, w, i) * d) - t * k;
+        };
+        for (int i = lane; i < half_r; i += 32) {
+          int p, q;
+          float dp, dq;
+          pair_at(i, p, q);
+          turned_back(i, p, q, dp, dq);
+          dp = finish(p, dp), dq = finish(q, dq);
+          y[p] = from_float<T>(dp), y[q] = from_float<T>(dq);
+        }
+        for (int i = a.r + lane; i < a.D; i += 32) y[i] = from_float<T>(finish(i, to_float(dy[i])));
+      } else {
+        auto normed = [&](int i) {
+          return a.norm ? to_float(x[i]) * rstd * load_gamma(a, w, i) : to_float(x[i]);
+        };
+        for (int i = lane; i < half_r; i += 32) {
+          int p, q;
+          pair_at(i, p, q);
+          const float u = normed(p), v = normed(q);
+          y[p] = from_float<T>(u * table[i].x - v * table[i].y);
+          y[q] = from_float<T>(v * table[i].x + u * table[i].y);
+        }
+        for (int i = a.r + lane; i < a.D; i += 32) y[i] = from_float<T>(normed(i));
+      }
+    }
+  }
+  if (kBwd && a.partial != nullptr) {
+    __syncthreads();
+    const float* all = reinterpret_cast<const float*>(table + half_r);
+    for (int i = threadIdx.x; i < a.D; i += kThreads) {
+      float t = 0.f;
+      for (int k = 0; k < kWarps; ++k) t += all[k * a.D + i];
+      a.partial[static_cast<int64_t>(blockIdx.x) * a.D + i] = t;
+    }
+  }
+}
+
+// dgamma[w][c] = sum over the CTAs of queries (w = 0) or keys (w = 1), in a fixed order: 8 interleaved sums in 64 bits
+__global__ void __launch_bounds__(256) dgamma_kernel(const float* partial, int q_ctas, int ctas, int D, float* dq_gamma,
+                                                     float* dk_gamma) {
+  __shared__ double red[8][32];
+  const int c = blockIdx.x * 32 + (threadIdx.x & 31), part = threadIdx.x >> 5;
+  const int lo = blockIdx.y ? q_ctas : 0, hi = blockIdx.y ? ctas : q_ctas;
+  float* out = blockIdx.y ? dk_gamma : dq_gamma;
+  double t = 0.0;
+  if (c < D)
+    for (int i = lo + part; i < hi; i += 8) t += partial[static_cast<int64_t>(i) * D + c];
+  red[part][threadIdx.x & 31] = t;
+  __syncthreads();
+  if (part == 0 && c < D && out != nullptr) {
+    for (int k = 1; k < 8; ++k) t += red[k][threadIdx.x & 31];
+    out[c] = static_cast<float>(t);
+  }
+}
+
+// ------------------------------------------------ host ---------------------------------------------------------
+int64_t type_size(int32_t dtype) { return dtype == 2 ? 4 : 2; }
+
+struct Problem {
+  int64_t B, S, H[2], D, r;
+  int32_t dtype;
+};
+
+// Fills an operand; a stride of a dimension of one element is never used and is read as 0.
+Operand operand(const void* p, const int64_t* strides, const Problem& pr, int w) {
+  return {const_cast<void*>(p), pr.B > 1 ? strides[0] : 0, pr.S > 1 ? strides[1] : 0, pr.H[w] > 1 ? strides[2] : 0};
+}
+
+// Elements of an output must not share memory: no stride of 0 over several elements.
+bool writes_apart(const Operand& o, const Problem& pr, int w) {
+  return (pr.B <= 1 || o.b != 0) && (pr.S <= 1 || o.s != 0) && (pr.H[w] <= 1 || o.h != 0);
+}
+
+bool is_vector_operand(const Operand& o, int64_t E) {
+  return aschost::aligned16(o.p) && o.b % E == 0 && o.s % E == 0 && o.h % E == 0;
+}
+
+// Checks shared by both directions; *done: there is nothing to compute.
+int32_t check(const int64_t* dims, const int64_t* strides, const void* positions, const double* freq, int32_t dtype,
+              int32_t gamma_dtype, int32_t flags, Problem& pr, bool* done) {
+  *done = false;
+  if (dims == nullptr || strides == nullptr) return ASC_ERR_INVALID_ARG;
+  pr = {dims[0], dims[1], {dims[2], dims[3]}, dims[4], dims[5], dtype};
+  if (dtype < 0 || dtype > 2 || gamma_dtype < 0 || gamma_dtype > 2 || (flags & ~15) != 0) return ASC_ERR_INVALID_ARG;
+  if (pr.B < 0 || pr.S < 0 || pr.H[0] < 0 || pr.H[1] < 0 || pr.D < 0 || pr.r < 0 || pr.r > pr.D || pr.r % 2 != 0)
+    return ASC_ERR_INVALID_ARG;
+  if (pr.D > kMaxHeadDim || pr.H[0] > 0x100000 || pr.H[1] > 0x100000) return ASC_ERR_TOO_LARGE;
+  if (pr.B == 0 || pr.S == 0 || pr.D == 0 || pr.H[0] + pr.H[1] == 0) {
+    *done = true;
+    return ASC_OK;
+  }
+  // token numbers stay below 2^30, so that rounding them up to a chunk cannot pass 32 bits
+  if (pr.S > (1 << 30) || pr.B > (1 << 30) || pr.B * pr.S > (1 << 30)) return ASC_ERR_TOO_LARGE;
+  if (pr.r > 0 && (positions == nullptr || freq == nullptr)) return ASC_ERR_INVALID_ARG;
+  const uintptr_t pos_align = (flags & 4) ? 4 : 8;
+  if (reinterpret_cast<uintptr_t>(positions) % pos_align != 0 || reinterpret_cast<uintptr_t>(freq) % 8 != 0)
+    return ASC_ERR_MISALIGNED;
+  return ASC_OK;
+}
+
+void fill(RotaryArgs& a, const Problem& pr, const int64_t* pos_strides, const void* positions, const double* freq,
+          float eps, float scale, int32_t gamma_dtype, int32_t flags) {
+  a.positions = positions;
+  a.freq = freq;
+  a.pos_b = pr.B > 1 ? pos_strides[0] : 0;
+  a.pos_s = pr.S > 1 ? pos_strides[1] : 0;
+  a.S = static_cast<int32_t>(pr.S);
+  a.tokens = static_cast<int32_t>(pr.B * pr.S);
+  a.heads[0] = static_cast<int32_t>(pr.H[0]);
+  a.heads[1] = static_cast<int32_t>(pr.H[1]);
+  a.D = static_cast<int32_t>(pr.D);
+  a.r = static_cast<int32_t>(pr.r);
+  a.interleaved = flags & 1;
+  a.norm = (flags >> 1) & 1;
+  a.pos32 = (flags >> 2) & 1;
+  a.conj = (flags >> 3) & 1;
+  a.gamma_type = gamma_dtype;
+  a.eps = eps;
+  a.scale = scale;
+}
+
+// Lanes per row of the vector kernels, as a power of two; 0 when they do not apply.
+int vector_lanes(const Problem& pr, int interleaved) {
+  const int64_t E = 16 / type_size(pr.dtype);
+  if (pr.D % E != 0 || (!interleaved && (pr.r / 2) % E != 0)) return 0;
+  const int64_t n = pr.D / E, hv = pr.r / 2 / E;
+  const int64_t units = interleaved ? (n + 1) / 2 : hv + (n - 2 * hv + 1) / 2;
+  if (units > 32) return 0;
+  int lanes = 4;
+  while (lanes < units) lanes *= 2;
+  return lanes;
+}
+
+int log2_of(int64_t v) {
+  int l = 0;
+  while ((int64_t{1} << (l + 1)) <= v) ++l;
+  return l;
+}
+
+template <typename T>
+int32_t launch_fwd(RotaryArgs a, const Problem& pr, cudaStream_t st) {
+  int sms = 0;
+  int32_t rc = aschost::sm_count(&sms);
+  if (rc != ASC_OK) return rc;
+  constexpr int E = Vec<T>::E;
+  const int64_t tokens = a.tokens;
+  const int H = a.heads[0] + a.heads[1];
+  int lanes = vector_lanes(pr, a.interleaved);
+  for (int w = 0; w < 2; ++w)
+    if (pr.H[w] > 0 && !(is_vector_operand(a.x[w], E) && is_vector_operand(a.y[w], E))) lanes = 0;
+  if (lanes == 0) {
+    const int64_t grid = tokens < sms * 8ll ? tokens : sms * 8ll;
+    rotary_any_kernel<T, false><<<static_cast<unsigned>(grid), kThreads, a.r / 2 * sizeof(float2), st>>>(a);
+  } else {
+    const int groups = kThreads / lanes;
+    // Tokens per CTA: enough rows for every group (about two each), but no fewer CTAs than SMs.
+    int log_t = log2_of(groups);
+    while (log_t > 0 && ((tokens + (1 << log_t) - 1) >> log_t) < 4ll * sms) --log_t;
+    while (log_t > 0 && (groups >> log_t) < 2 && H > 4) --log_t;
+    a.log_lanes = log2_of(lanes);
+    a.log_tokens = log_t;
+    const int per_token = groups >> log_t;
+    // one token per CTA: its heads are spread over more CTAs when few tokens would leave SMs idle
+    int64_t y = 1;
+    if (log_t == 0) {
+      y = (H + per_token - 1) / per_token;
+      if (tokens * y > 2ll * sms) y = 1;
+    }
+    const dim3 grid(static_cast<unsigned>((tokens + (1 << log_t) - 1) >> log_t), static_cast<unsigned>(y));
+    const size_t smem = (size_t{1} << log_t) * (a.r / 2) * sizeof(float2);
+    if (a.norm) {
+      if (a.interleaved) rotary_fwd_kernel<T, true, true><<<grid, kThreads, smem, st>>>(a);
+      else rotary_fwd_kernel<T, true, false><<<grid, kThreads, smem, st>>>(a);
+    } else {
+      if (a.interleaved) rotary_fwd_kernel<T, false, true><<<grid, kThreads, smem, st>>>(a);
+      else rotary_fwd_kernel<T, false, false><<<grid, kThreads, smem, st>>>(a);
+    }
+  }
+  aschost::count_launch();
+  ASC_CUDA_TRY(cudaGetLastError());
+  return ASC_OK;
+}
+
+template <typename T>
+int32_t launch_bwd(RotaryArgs a, const Problem& pr, float* dq_gamma, float* dk_gamma, cudaStream_t st) {
+  int sms = 0;
+  int32_t rc = aschost::sm_count(&sms);
+  if (rc != ASC_OK) return rc;
+  constexpr int E = Vec<T>::E;
+  int lanes = vector_lanes(pr, a.interleaved);
+  for (int w = 0; w < 2; ++w)
+    if (pr.H[w] > 0 && !(is_vector_operand(a.x[w], E) && is_vector_operand(a.y[w], E) && is_vector_operand(a.dy[w], E)))
+      lanes = 0;
+  int log_t = 0;
+  if (lanes != 0) {
+    const int groups = kThreads / lanes;
+    log_t = log2_of(groups);
+    while (log_t > 0 && ((static_cast<int64_t>(a.tokens) + (1 << log_t) - 1) >> log_t) < 4ll * sms) --log_t;
+    while (log_t > 0 && (groups >> log_t) < 2 && a.heads[0] > 4) --log_t;
+    a.log_lanes = log2_of(lanes);
+    a.log_tokens = log_t;
+  }
+  // CTAs of queries and of keys in the ratio of their heads, at least one each where there are heads
+  const int64_t chunks = (static_cast<int64_t>(a.tokens) + (1 << log_t) - 1) >> log_t;
+  const int64_t slots = 2ll * sms, H = pr.H[0] + pr.H[1];
+  int64_t ctas[2];
+  for (int w = 0; w < 2; ++w) {
+    ctas[w] = slots * pr.H[w] / H;
+    if (ctas[w] == 0 && pr.H[w] > 0) ctas[w] = 1;
+    if (ctas[w] > chunks) ctas[w] = chunks;
+  }
+  a.q_ctas = static_cast<int32_t>(ctas[0]);
+  const int64_t grid = ctas[0] + ctas[1];
+  void* ws = nullptr;
+  if (dq_gamma != nullptr || dk_gamma != nullptr) {
+    if ((rc = aschost::scratch_alloc(&ws, static_cast<size_t>(grid) * a.D * sizeof(float), st)) != ASC_OK) return rc;
+    a.partial = static_cast<float*>(ws);
+  }
+  if (lanes == 0) {
+    const size_t smem = a.r / 2 * sizeof(float2) + static_cast<size_t>(kWarps) * a.D * sizeof(float);
+    rotary_any_kernel<T, true><<<static_cast<unsigned>(grid), kThreads, smem, st>>>(a);
+  } else {
+    const size_t smem = (size_t{1} << log_t) * (a.r / 2) * sizeof(float2);
+    if (a.interleaved) rotary_bwd_kernel<T, true><<<static_cast<unsigned>(grid), kThreads, smem, st>>>(a);
+    else rotary_bwd_kernel<T, false><<<static_cast<unsigned>(grid), kThreads, smem, st>>>(a);
+  }
+  cudaError_t e = cudaGetLastError();
+  if (e == cudaSuccess) {
+    aschost::count_launch();
+    if (ws != nullptr) {
+      dgamma_kernel<<<dim3((a.D + 31) / 32, 2), 256, 0, st>>>(a.partial, a.q_ctas, static_cast<int>(grid), a.D, dq_gamma,
+                                                              dk_gamma);
+      e = cudaGetLastError();
+      if (e == cudaSuccess) aschost::count_launch();
+    }
+  }
+  if (ws != nullptr) {
+    rc = aschost::scratch_free(ws, st);
+    if (e == cudaSuccess && rc != ASC_OK) return rc;
+  }
+  ASC_CUDA_TRY(e);
+  return ASC_OK;
+}
+
+}  // namespace
+
+extern "C" int32_t asc_cuda_norm_rotary(const void* q, const void* k, void* q_out, void* k_out, const void* q_gamma,
+                                        const void* k_gamma, const void* positions, const double* frequencies,
+                                        const int64_t* dims, const int64_t* strides, float eps, float scale,
+                                        int32_t dtype, int32_t gamma_dtype, int32_t flags, void* stream) {
+  Problem pr;
+  bool done;
+  const int32_t rc = check(dims, strides, positions, frequencies, dtype, gamma_dtype, flags, pr, &done);
+  if (rc != ASC_OK || done) return rc;
+  const void* in[2] = {q, k};
+  void* out[2] = {q_out, k_out};
+  const void* gamma[2] = {q_gamma, k_gamma};
+  RotaryArgs a{};
+  fill(a, pr, strides + 12, positions, frequencies, eps, scale, gamma_dtype, flags);
+  for (int w = 0; w < 2; ++w) {
+    if (pr.H[w] == 0) continue;
+    if (in[w] == nullptr || out[w] == nullptr) return ASC_ERR_INVALID_ARG;
+    if (reinterpret_cast<uintptr_t>(in[w]) % type_size(dtype) != 0 || reinterpret_cast<uintptr_t>(out[w]) % type_size(dtype) != 0)
+      return ASC_ERR_MISALIGNED;
+    if (a.norm && reinterpret_cast<uintptr_t>(gamma[w]) % type_size(gamma_dtype) != 0) return ASC_ERR_MISALIGNED;
+    a.x[w] = operand(in[w], strides + 3 * w, pr, w);
+    a.y[w] = operand(out[w], strides + 6 + 3 * w, pr, w);
+    a.gamma[w] = gamma[w];
+    if (!writes_apart(a.y[w], pr, w)) return ASC_ERR_INVALID_ARG;
+  }
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (dtype == 0) return launch_fwd<__half>(a, pr, st);
+  if (dtype == 1) return launch_fwd<__nv_bfloat16>(a, pr, st);
+  return launch_fwd<float>(a, pr, st);
+}
+
+extern "C" int32_t asc_cuda_norm_rotary_bwd(const void* dq_out, const void* dk_out, const void* q, const void* k, void* dq,
+                                            void* dk, const void* q_gamma, const void* k_gamma, float* dq_gamma,
+                                            float* dk_gamma, const void* positions, const double* frequencies,
+                                            const int64_t* dims, const int64_t* strides, float eps, float scale,
+                                            int32_t dtype, int32_t gamma_dtype, int32_t flags, void* stream) {
+  Problem pr;
+  bool done;
+  const int32_t rc = check(dims, strides, positions, frequencies, dtype, gamma_dtype, flags, pr, &done);
+  if (rc != ASC_OK) return rc;
+  if ((flags & 10) != 2) return ASC_ERR_INVALID_ARG;      // norm, not turned back: see the header
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  float* dgamma[2] = {dq_gamma, dk_gamma};
+  for (int w = 0; w < 2; ++w) {                           // a sum over no rows
+    if (dgamma[w] == nullptr) continue;
+    if (reinterpret_cast<uintptr_t>(dgamma[w]) % 4 != 0) return ASC_ERR_MISALIGNED;
+    if (done && pr.D > 0) ASC_CUDA_TRY(cudaMemsetAsync(dgamma[w], 0, pr.D * sizeof(float), st));
+  }
+  if (done) return ASC_OK;
+  const void* g_in[2] = {dq_out, dk_out};
+  const void* in[2] = {q, k};
+  void* out[2] = {dq, dk};
+  const void* gamma[2] = {q_gamma, k_gamma};
+  const uintptr_t size = type_size(dtype);
+  RotaryArgs a{};
+  fill(a, pr, strides + 18, positions, frequencies, eps, scale, gamma_dtype, flags);
+  for (int w = 0; w < 2; ++w) {
+    if (pr.H[w] == 0) continue;
+    if (in[w] == nullptr || out[w] == nullptr || g_in[w] == nullptr) return ASC_ERR_INVALID_ARG;
+    if (reinterpret_cast<uintptr_t>(in[w]) % size != 0 || reinterpret_cast<uintptr_t>(out[w]) % size != 0 ||
+        reinterpret_cast<uintptr_t>(g_in[w]) % size != 0 ||
+        reinterpret_cast<uintptr_t>(gamma[w]) % type_size(gamma_dtype) != 0)
+      return ASC_ERR_MISALIGNED;
+    a.dy[w] = operand(g_in[w], strides + 3 * w, pr, w);
+    a.x[w] = operand(in[w], strides + 6 + 3 * w, pr, w);
+    a.y[w] = operand(out[w], strides + 12 + 3 * w, pr, w);
+    a.gamma[w] = gamma[w];
+    if (!writes_apart(a.y[w], pr, w)) return ASC_ERR_INVALID_ARG;
+  }
+  if (dtype == 0) return launch_bwd<__half>(a, pr, dgamma[0], dgamma[1], st);
+  if (dtype == 1) return launch_bwd<__nv_bfloat16>(a, pr, dgamma[0], dgamma[1], st);
+  return launch_bwd<float>(a, pr, dgamma[0], dgamma[1], st);
+}
