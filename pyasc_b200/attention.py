@@ -11,9 +11,8 @@ a packed projection, or ``x.transpose(1, 2)`` of a [batch, heads, sequence, head
 """
 from __future__ import annotations
 
-import contextlib
-import ctypes
 import math
+import struct
 from typing import Optional, Sequence, Tuple
 
 import torch
@@ -26,47 +25,65 @@ _DTYPE_CODE = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}
 # --------------------------------------------------------------------------------------------------
 # Arguments
 # --------------------------------------------------------------------------------------------------
-def _check_tensor(name: str, t: torch.Tensor, dtypes: Sequence[torch.dtype], device: Optional[torch.device],
-                  shape: Optional[Sequence[int]] = None) -> None:
+# A call's host time is a large part of the smallest launches: the checks read each property of a tensor once and
+# leave the wording of an error to the second look.
+def _device_of(name: str, t: torch.Tensor) -> int:
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{name} must be a torch tensor, got {type(t).__name__}")
     if not t.is_cuda:
         raise ValueError(f"{name} must be a CUDA tensor")
-    if device is not None and t.device != device:
-        raise ValueError(f"{name} is on {t.device}, expected {device}")
+    return t.get_device()
+
+
+def _check_rows(name: str, t: torch.Tensor, dtype: torch.dtype, device: int) -> Tuple[int, ...]:
+    """Shape of a [batch, sequence, heads, head_dim] tensor of this type and device."""
+    if _device_of(name, t) != device:
+        raise ValueError(f"{name} is on {t.device}, expected cuda:{device}")
+    if t.dtype != dtype:
+        raise TypeError(f"{name} has type {t.dtype}, expected {dtype}")
+    shape = t.shape
+    if len(shape) != 4:
+        raise ValueError(f"{name} must be [batch, sequence, heads, head_dim], got {len(shape)} dimensions")
+    if shape[3] > 1 and t.stride(3) != 1:
+        raise ValueError(f"the last dimension of {name} must be contiguous")
+    return shape
+
+
+def _check_shape(name: str, shape: Sequence[int], expected: Sequence[int]) -> None:
+    if shape != expected:
+        raise ValueError(f"{name} has shape {tuple(shape)}, expected {tuple(expected)}")
+
+
+def _check_vector(name: str, t: torch.Tensor, dtypes, device: int) -> None:
+    """A tensor of one of these types on this device."""
+    if _device_of(name, t) != device:
+        raise ValueError(f"{name} is on {t.device}, expected cuda:{device}")
     if t.dtype not in dtypes:
         raise TypeError(f"{name} has type {t.dtype}, expected {' or '.join(str(d) for d in dtypes)}")
-    if shape is not None and tuple(t.shape) != tuple(shape):
-        raise ValueError(f"{name} has shape {tuple(t.shape)}, expected {tuple(shape)}")
 
 
-def _check_rows(name: str, t: torch.Tensor) -> None:
-    if t.dim() != 4:
-        raise ValueError(f"{name} must be [batch, sequence, heads, head_dim], got {t.dim()} dimensions")
-    if t.shape[3] > 1 and t.stride(3) != 1:
-        raise ValueError(f"the last dimension of {name} must be contiguous")
-
-
-def _check_output(name: str, t: torch.Tensor, like: torch.Tensor, shape: Sequence[int]) -> None:
-    _check_tensor(name, t, (like.dtype, ), like.device, shape)
-    _check_rows(name, t)
-    if any(n > 1 and s == 0 for n, s in zip(t.shape, t.stride())):
+def _output(name: str, given: Optional[torch.Tensor], like: torch.Tensor, shape: Sequence[int], device: int) -> torch.Tensor:
+    """The given output, checked, or a new one (in the order of ``like``'s dimensions)."""
+    if given is None:
+        return torch.empty_like(like)
+    _check_shape(name, _check_rows(name, given, like.dtype, device), shape)
+    if any(n > 1 and s == 0 for n, s in zip(given.shape, given.stride())):
         raise ValueError(f"{name} repeats memory (a stride of 0): it cannot be written")
+    return given
 
 
-def _ptr(t: Optional[torch.Tensor]) -> Optional[int]:
-    return None if t is None else t.data_ptr()
+_PACK = {n: struct.Struct(f"{n}q").pack for n in (6, 14, 20)}     # host int64 arrays of the C ABI
+_NO_STRIDES = (0, 0, 0)
 
 
-def _int64s(*values: int):
-    return (ctypes.c_int64 * len(values))(*values)
-
-
-def _call(fn_name: str, device: torch.device, *args) -> None:
+def _call(fn_name: str, device: int, *args) -> None:
     """One C-ABI call with ``device`` current, on its current torch stream."""
-    index = device.index
-    with contextlib.nullcontext() if index == torch.cuda.current_device() else torch.cuda.device(index):
-        capi.call(fn_name, *args, torch.cuda.current_stream(index).cuda_stream)
+    stream = torch._C._cuda_getCurrentRawStream(device)
+    if device == torch.cuda.current_device():
+        capi.call(fn_name, *args, stream)
+    else:
+        with torch.cuda.device(device):
+            capi.call(fn_name, *args, stream)
 
 
 # --------------------------------------------------------------------------------------------------
@@ -111,44 +128,53 @@ def rotary_frequencies(rotated: int, base: float = 10000.0, *, scaling: Optional
 
 
 def _rotary_arguments(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor, frequencies: torch.Tensor):
-    """Checks what all four functions share; dims, strides of the positions and the flag of their type."""
-    _check_tensor("q", q, tuple(_DTYPE_CODE), None)
-    _check_rows("q", q)
-    batch, seq, heads, head_dim = q.shape
-    kv_heads = 0
+    """Checks what all four functions share: device, shapes, the C ABI's dims, strides and type flag of the positions."""
+    device = _device_of("q", q)
+    dtype = q.dtype
+    if dtype not in _DTYPE_CODE:
+        raise TypeError(f"q has type {dtype}, expected float16, bfloat16 or float32")
+    q_shape = _check_rows("q", q, dtype, device)
+    batch, seq, heads, head_dim = q_shape
+    kv_heads, k_shape = 0, None
     if k is not None:
-        _check_tensor("k", k, (q.dtype, ), q.device)
-        _check_rows("k", k)
-        kv_heads = k.shape[2]
-        if k.shape != (batch, seq, kv_heads, head_dim):
-            raise ValueError(f"k has shape {tuple(k.shape)}, q {tuple(q.shape)}: only the heads may differ")
-    _check_tensor("positions", positions, (torch.int64, torch.int32), q.device)
-    if positions.dim() not in (1, 2) or positions.shape[-1] != seq or (positions.dim() == 2 and
-                                                                       positions.shape[0] not in (1, batch)):
-        raise ValueError(f"positions must be [sequence] or [batch, sequence], got {tuple(positions.shape)}")
-    _check_tensor("frequencies", frequencies, (torch.float64, ), q.device)
-    if frequencies.dim() != 1 or (frequencies.numel() > 1 and frequencies.stride(0) != 1):
+        k_shape = _check_rows("k", k, dtype, device)
+        kv_heads = k_shape[2]
+        _check_shape("k", k_shape, (batch, seq, kv_heads, head_dim))
+    _check_vector("positions", positions, _POSITION_TYPES, device)
+    shape, pos_strides = positions.shape, positions.stride()
+    if len(shape) == 1 and shape[0] == seq:
+        pos_strides = (0, pos_strides[0])
+    elif len(shape) == 2 and shape[1] == seq and shape[0] in (1, batch):
+        if shape[0] == 1:
+            pos_strides = (0, pos_strides[1])
+    else:
+        raise ValueError(f"positions must be [sequence] or [batch, sequence], got {tuple(shape)}")
+    _check_vector("frequencies", frequencies, _FREQUENCY_TYPES, device)
+    if frequencies.dim() != 1 or not frequencies.is_contiguous():
         raise ValueError("frequencies must be one contiguous row")
     rotated = 2 * frequencies.numel()
     if rotated > head_dim:
         raise ValueError(f"{frequencies.numel()} frequencies turn {rotated} elements of a head of {head_dim}")
-    batch_stride = positions.stride(0) if positions.dim() == 2 and positions.shape[0] > 1 else 0
     flags = 4 if positions.dtype == torch.int32 else 0
-    return (batch, seq, heads, kv_heads, head_dim, rotated), (batch_stride, positions.stride(-1)), flags
+    return device, q_shape, k_shape, _PACK[6](batch, seq, heads, kv_heads, head_dim, rotated), pos_strides, flags
 
 
-def _strides(t: Optional[torch.Tensor]) -> Tuple[int, int, int]:
-    return (0, 0, 0) if t is None else t.stride()[:3]
+_POSITION_TYPES = (torch.int64, torch.int32)
+_FREQUENCY_TYPES = (torch.float64, )
 
 
-def _gammas(q: torch.Tensor, k: Optional[torch.Tensor], q_gamma: Optional[torch.Tensor],
-            k_gamma: Optional[torch.Tensor]) -> int:
+def _strides(t: Optional[torch.Tensor]) -> Tuple[int, ...]:
+    return _NO_STRIDES if t is None else t.stride()[:3]
+
+
+def _gammas(device: int, head_dim: int, q_gamma: Optional[torch.Tensor], k_gamma: Optional[torch.Tensor]) -> int:
     code = None
     for name, g in (("q_gamma", q_gamma), ("k_gamma", k_gamma)):
         if g is None:
             continue
-        _check_tensor(name, g, tuple(_DTYPE_CODE), q.device, (q.shape[3], ))
-        if g.numel() > 1 and g.stride(0) != 1:
+        _check_vector(name, g, _DTYPE_CODE, device)
+        _check_shape(name, g.shape, (head_dim, ))
+        if not g.is_contiguous():
             raise ValueError(f"{name} must be contiguous")
         if code is not None and code != _DTYPE_CODE[g.dtype]:
             raise TypeError("q_gamma and k_gamma must have one type")
@@ -157,24 +183,21 @@ def _gammas(q: torch.Tensor, k: Optional[torch.Tensor], q_gamma: Optional[torch.
 
 
 def _rotate(q, k, q_gamma, k_gamma, positions, frequencies, eps, scale, interleaved, flags, q_out, k_out):
-    dims, pos_strides, pos_flag = _rotary_arguments(q, k, positions, frequencies)
-    gamma_code = _gammas(q, k, q_gamma, k_gamma)
-    if q_out is None:
-        q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    else:
-        _check_output("q_out", q_out, q, q.shape)
-    if k is None:
-        if k_out is not None:
-            raise ValueError("k_out without k")
-    elif k_out is None:
-        k_out = torch.empty(k.shape, dtype=k.dtype, device=k.device)
-    else:
-        _check_output("k_out", k_out, k, k.shape)
-    _call("asc_cuda_norm_rotary", q.device, _ptr(q), _ptr(k), _ptr(q_out), _ptr(k_out), _ptr(q_gamma), _ptr(k_gamma),
-          _ptr(positions), _ptr(frequencies), _int64s(*dims),
-          _int64s(*_strides(q), *_strides(k), *_strides(q_out), *_strides(k_out), *pos_strides), eps, scale,
+    device, q_shape, k_shape, dims, pos_strides, pos_flag = _rotary_arguments(q, k, positions, frequencies)
+    if k is None and (k_out is not None or k_gamma is not None):
+        raise ValueError("an output or a gamma of k without k")
+    gamma_code = 0 if q_gamma is None and k_gamma is None else _gammas(device, q_shape[3], q_gamma, k_gamma)
+    q_out = _output("the output of q", q_out, q, q_shape, device)
+    k_out = None if k is None else _output("the output of k", k_out, k, k_shape, device)
+    _call("asc_cuda_norm_rotary", device, q.data_ptr(), _ptr(k), q_out.data_ptr(), _ptr(k_out), _ptr(q_gamma),
+          _ptr(k_gamma), positions.data_ptr(), frequencies.data_ptr(), dims,
+          _PACK[14](*_strides(q), *_strides(k), *_strides(q_out), *_strides(k_out), *pos_strides), eps, scale,
           _DTYPE_CODE[q.dtype], gamma_code, flags | pos_flag | bool(interleaved))
     return q_out, k_out
+
+
+def _ptr(t: Optional[torch.Tensor]) -> Optional[int]:
+    return None if t is None else t.data_ptr()
 
 
 def rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor, frequencies: torch.Tensor, *,
@@ -211,31 +234,21 @@ def norm_rotary_backward(dq_out: torch.Tensor, dk_out: Optional[torch.Tensor], q
     """Gradients ``(dq, dk, dq_gamma, dk_gamma)`` of :func:`norm_rotary` from those of its outputs and its inputs.  The
     gammas' gradients are float32 sums over all rows in a fixed order (None where there is no gamma).  ``dq`` may be
     ``dq_out`` or ``q``, ``dk`` likewise."""
-    dims, pos_strides, pos_flag = _rotary_arguments(q, k, positions, frequencies)
-    gamma_code = _gammas(q, k, q_gamma, k_gamma)
-    _check_tensor("dq_out", dq_out, (q.dtype, ), q.device, q.shape)
-    _check_rows("dq_out", dq_out)
+    device, q_shape, k_shape, dims, pos_strides, pos_flag = _rotary_arguments(q, k, positions, frequencies)
     if (k is None) != (dk_out is None):
         raise ValueError("k and dk_out go together")
-    if dq is None:
-        dq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    else:
-        _check_output("dq", dq, q, q.shape)
-    if k is None:
-        if dk is not None or k_gamma is not None:
-            raise ValueError("dk or k_gamma without k")
-    else:
-        _check_tensor("dk_out", dk_out, (k.dtype, ), k.device, k.shape)
-        _check_rows("dk_out", dk_out)
-        if dk is None:
-            dk = torch.empty(k.shape, dtype=k.dtype, device=k.device)
-        else:
-            _check_output("dk", dk, k, k.shape)
-    dq_gamma, dk_gamma = (None if g is None else torch.empty(q.shape[3], dtype=torch.float32, device=q.device)
-                          for g in (q_gamma, k_gamma))
-    _call("asc_cuda_norm_rotary_bwd", q.device, _ptr(dq_out), _ptr(dk_out), _ptr(q), _ptr(k), _ptr(dq), _ptr(dk),
-          _ptr(q_gamma), _ptr(k_gamma), _ptr(dq_gamma), _ptr(dk_gamma), _ptr(positions), _ptr(frequencies),
-          _int64s(*dims),
-          _int64s(*_strides(dq_out), *_strides(dk_out), *_strides(q), *_strides(k), *_strides(dq), *_strides(dk),
-                  *pos_strides), eps, scale, _DTYPE_CODE[q.dtype], gamma_code, 2 | pos_flag | bool(interleaved))
+    if k is None and (dk is not None or k_gamma is not None):
+        raise ValueError("an output or a gamma of k without k")
+    gamma_code = _gammas(device, q_shape[3], q_gamma, k_gamma)
+    _check_shape("dq_out", _check_rows("dq_out", dq_out, q.dtype, device), q_shape)
+    dq = _output("dq", dq, q, q_shape, device)
+    if k is not None:
+        _check_shape("dk_out", _check_rows("dk_out", dk_out, q.dtype, device), k_shape)
+        dk = _output("dk", dk, k, k_shape, device)
+    dq_gamma, dk_gamma = (None if g is None else torch.empty_like(g, dtype=torch.float32) for g in (q_gamma, k_gamma))
+    _call("asc_cuda_norm_rotary_bwd", device, dq_out.data_ptr(), _ptr(dk_out), q.data_ptr(), _ptr(k), dq.data_ptr(),
+          _ptr(dk), _ptr(q_gamma), _ptr(k_gamma), _ptr(dq_gamma), _ptr(dk_gamma), positions.data_ptr(),
+          frequencies.data_ptr(), dims,
+          _PACK[20](*_strides(dq_out), *_strides(dk_out), *_strides(q), *_strides(k), *_strides(dq), *_strides(dk),
+                    *pos_strides), eps, scale, _DTYPE_CODE[q.dtype], gamma_code, 2 | pos_flag | bool(interleaved))
     return dq, dk, dq_gamma, dk_gamma

@@ -41,7 +41,7 @@ struct RotaryArgs {
   int32_t heads[2];
   int32_t D, r;
   int32_t log_lanes;       // lanes per row (vector kernels)
-  int32_t log_tokens;      // tokens a CTA works on at a time
+  int32_t slices;          // parts a token's heads are cut into, one warp each (vector kernels)
   int32_t q_ctas;          // backward: CTAs [0, q_ctas) own queries, the others keys
   int32_t gamma_type;      // 0 fp16, 1 bf16, 2 fp32
   int32_t pos32;           // positions are int32 instead of int64
@@ -123,16 +123,13 @@ __device__ __forceinline__ float load_gamma(const RotaryArgs& a, int which, int 
   return static_cast<const float*>(g)[i];
 }
 
-// scale * (cos, sin) of the angle of `token`'s pair `f`; `conj` turns back
-__device__ __forceinline__ float2 turn_of(const RotaryArgs& a, int token, int f) {
-  const int b = token / a.S, s = token - b * a.S;
-  const int64_t at = b * a.pos_b + s * a.pos_s;
-  const double pos = a.pos32 ? static_cast<double>(static_cast<const int32_t*>(a.positions)[at])
-                             : static_cast<double>(static_cast<const int64_t*>(a.positions)[at]);
+// scale * (cos, sin) of the angle of pair `f` at position `pos`; `conj` turns back
+__device__ __forceinline__ float2 turn_of(const RotaryArgs& a, double pos, int f) {
   // turns = pos * f / (2 pi) as a rounded value and what the roundings left out, so that the fraction of a turn is
   // right to 2^-50 at any position (in plain 64 bits it would be off by 2^-16 of a turn at position 2^40)
   constexpr double kInv2Pi = 0.15915494309189535, kInv2PiRest = -9.839338337591243e-18;
-  const double angle = pos * a.freq[f], angle_rest = fma(pos, a.freq[f], -angle);
+  const double frequency = a.freq[f];
+  const double angle = pos * frequency, angle_rest = fma(pos, frequency, -angle);
   const double turns = angle * kInv2Pi;
   const double rest = fma(angle, kInv2Pi, -turns) + (angle * kInv2PiRest + angle_rest * kInv2Pi);
   float sn, cs;
@@ -169,43 +166,71 @@ struct LaneVectors {
   }
 };
 
-// cos / sin of the pairs a lane owns, as fp32 registers.  Interleaved: the first E / 2 belong to vector v0.
+// Coefficients of a lane's rotation, as pairs of fp32 registers (packed arithmetic halves the instructions).  Half layout,
+// E pairs of elements (x_lo[e], x_hi[e]):  y_lo = lo_lo x_lo + lo_hi x_hi,  y_hi = hi_hi x_hi + hi_lo x_lo,  with the
+// gammas multiplied in once per token.  Interleaved: the same for the pair (v[2 e], v[2 e + 1]).
 template <int E>
-__device__ __forceinline__ void lane_turns(const RotaryArgs& a, const LaneVectors<E>& l, const float2* table, float* c,
-                                           float* s) {
-  const int half_r = a.r / 2;
+struct Turn {
+  float2 lo_lo[E / 2], lo_hi[E / 2], hi_hi[E / 2], hi_lo[E / 2];
+};
+
+template <int E>
+__device__ __forceinline__ float& at(float2 (&v)[E], int i) {
+  return (i & 1) ? v[i >> 1].y : v[i >> 1].x;
+}
+
+// index of the angle of the lane's pair e; r / 2 or more: not turned
+template <int E, bool kInter>
+__device__ __forceinline__ int angle_of(const RotaryArgs& a, const LaneVectors<E>& l, int e) {
+  if (kInter) return (e < E / 2 ? l.v0 : l.v1) * (E / 2) + (e & (E / 2 - 1));
+  return l.turns ? l.v0 * E + e : a.r / 2;
+}
+
+template <int E, bool kInter, bool kNorm>
+__device__ __forceinline__ void lane_turn(const RotaryArgs& a, const LaneVectors<E>& l, const float2* table,
+                                          const float* gamma, Turn<E>& t) {
 #pragma unroll
   for (int e = 0; e < E; ++e) {
-    int f;
-    if (a.interleaved)
-      f = (e < E / 2 ? l.v0 : l.v1) * (E / 2) + (e & (E / 2 - 1));
-    else
-      f = l.turns ? l.v0 * E + e : half_r;
-    const float2 t = f < half_r ? table[f] : make_float2(1.f, 0.f);
-    c[e] = t.x, s[e] = t.y;
+    const int f = angle_of<E, kInter>(a, l, e);
+    const float2 cs = f < a.r / 2 ? table[f] : make_float2(1.f, 0.f);
+    float g_lo = 1.f, g_hi = 1.f;
+    if (kNorm) {
+      // gammas of the two elements of pair e; elements past the end of the row read as 0 and are not stored
+      const int lo = kInter ? (e < E / 2 ? l.v0 : l.v1) * E + 2 * (e & (E / 2 - 1)) : l.v0 * E + e;
+      const int hi = kInter ? lo + 1 : l.v1 * E + e;
+      g_lo = lo < a.D ? gamma[lo] : 0.f;
+      g_hi = hi < a.D ? gamma[hi] : 0.f;
+    }
+    at(t.lo_lo, e) = g_lo * cs.x;
+    at(t.hi_hi, e) = g_hi * cs.x;
+    at(t.lo_hi, e) = -g_hi * cs.y;
+    at(t.hi_lo, e) = g_lo * cs.y;
   }
 }
 
-// Rotates the 2 E values of a lane in place.  Values that are not part of a pair are left alone, also non-finite ones.
+// Values that are not part of a pair are only scaled: their neighbours may be infinite or NaN.
 template <int E, bool kInter>
-__device__ __forceinline__ void rotate(const RotaryArgs& a, const LaneVectors<E>& l, const float* c, const float* s,
-                                       float* v, bool back) {
+__device__ __forceinline__ void apply(const RotaryArgs& a, const LaneVectors<E>& l, const Turn<E>& t, float2 (&v)[E]) {
   if (kInter) {
 #pragma unroll
     for (int e = 0; e < E; ++e) {
-      const int at = (e < E / 2 ? l.v0 : l.v1) * E + 2 * (e & (E / 2 - 1));
-      const float x = v[2 * e], y = v[2 * e + 1], sn = back ? -s[e] : s[e];
-      if (at < a.r) {
-        v[2 * e] = x * c[e] - y * sn;
-        v[2 * e + 1] = y * c[e] + x * sn;
-      }
+      const float2 x = v[e];
+      const bool turns = angle_of<E, kInter>(a, l, e) < a.r / 2;
+      const float lo = x.x * ((e & 1) ? t.lo_lo[e / 2].y : t.lo_lo[e / 2].x);
+      const float hi = x.y * ((e & 1) ? t.hi_hi[e / 2].y : t.hi_hi[e / 2].x);
+      v[e].x = turns ? fmaf(x.y, (e & 1) ? t.lo_hi[e / 2].y : t.lo_hi[e / 2].x, lo) : lo;
+      v[e].y = turns ? fmaf(x.x, (e & 1) ? t.hi_lo[e / 2].y : t.hi_lo[e / 2].x, hi) : hi;
     }
-  } else if (l.turns) {
+  } else {
 #pragma unroll
-    for (int e = 0; e < E; ++e) {
-      const float x = v[e], y = v[E + e], sn = back ? -s[e] : s[e];
-      v[e] = x * c[e] - y * sn;
-      v[E + e] = y * c[e] + x * sn;
+    for (int e = 0; e < E / 2; ++e) {
+      const float2 lo = v[e], hi = v[E / 2 + e];
+      v[e] = __fmul2_rn(lo, t.lo_lo[e]);
+      v[E / 2 + e] = __fmul2_rn(hi, t.hi_hi[e]);
+      if (l.turns) {
+        v[e] = __ffma2_rn(hi, t.lo_hi[e], v[e]);
+        v[E / 2 + e] = __ffma2_rn(lo, t.hi_lo[e], v[E / 2 + e]);
+      }
     }
   }
 }
@@ -215,126 +240,147 @@ __device__ __forceinline__ float group_sum(float v, int log_lanes) {
   return v;
 }
 
+__device__ __forceinline__ double position_at(const RotaryArgs& a, int b, int s) {
+  const int64_t i = b * a.pos_b + s * a.pos_s;
+  return a.pos32 ? static_cast<double>(static_cast<const int32_t*>(a.positions)[i])
+                 : static_cast<double>(static_cast<const int64_t*>(a.positions)[i]);
+}
+
+// Shared memory of the vector kernels: gammas of queries and keys as fp32 (D each, where there is a norm), then r / 2
+// angles for every warp.  Loads the gammas.
+__device__ __forceinline__ float2* stage(const RotaryArgs& a, float* smem) {
+  int floats = 0;
+  if (a.norm) {
+    for (int i = threadIdx.x; i < 2 * a.D; i += kThreads) smem[i] = load_gamma(a, i >= a.D, i >= a.D ? i - a.D : i);
+    floats = 2 * a.D;
+  }
+  __syncthreads();
+  return reinterpret_cast<float2*>(smem + floats) + (threadIdx.x >> 5) * (a.r / 2);
+}
+
 // --------------------------------------------------------------------------------------------------------------
-// Forward, whole 16-byte vectors.  A CTA works on 2^log_tokens tokens; the groups of a token share its heads, queries
-// first and then keys.  The next row is loaded before the current one is computed.
+// Forward, whole 16-byte vectors.  A warp works on one token, or on a slice of its heads where tokens are few: it
+// computes the token's angles into its own piece of shared memory (no barrier beyond the warp), then its groups of
+// lanes take the heads in turn, queries first and then keys.  The next row, also the next token's first, is loaded
+// before the current one is computed.  Warps stride over the tokens.
 // --------------------------------------------------------------------------------------------------------------
 template <typename T, bool kNorm, bool kInter>
 __global__ void __launch_bounds__(kThreads) rotary_fwd_kernel(const RotaryArgs a) {
   constexpr int E = Vec<T>::E;
-  extern __shared__ float2 table[];              // [tokens of this CTA][r / 2]
-  const int half_r = a.r / 2;
-  const int lane = threadIdx.x & ((1 << a.log_lanes) - 1), group = threadIdx.x >> a.log_lanes;
-  const int groups = kThreads >> a.log_lanes;
-  const int per_token = groups >> a.log_tokens;                 // groups that share a token
-  const int local = group / per_token;
-  const int token0 = blockIdx.x << a.log_tokens;
-  const int token = token0 + local;
+  extern __shared__ float smem[];
+  float2* table = stage(a, smem);
+  const int lane = threadIdx.x & ((1 << a.log_lanes) - 1), group = (threadIdx.x & 31) >> a.log_lanes;
+  const int groups = 32 >> a.log_lanes;
   const int H = a.heads[0] + a.heads[1];
-  const int step = per_token * gridDim.y;
-  const int first = blockIdx.y * per_token + (group - local * per_token);
+  const int step = groups * a.slices;
   const int iters = (H + step - 1) / step;
+  const int warps = gridDim.x * kWarps;
+  const int units = a.tokens * a.slices;
   const LaneVectors<E> l(a, lane);
-  const int b = token / a.S, s = token - b * a.S;
-  const bool here = token < a.tokens;
+  const float inv_d = 1.f / a.D;
 
-  auto load = [&](int h, uint4& lo, uint4& hi) {
+  struct Place {
+    int b, s, first;       // token and first head of this group
+  };
+  auto place = [&](int unit) {
+    const int token = unit / a.slices;
+    const int b = token / a.S;
+    return Place{b, token - b * a.S, (unit - token * a.slices) * groups + group};
+  };
+  auto load = [&](const Place& p, int h, uint4& lo, uint4& hi) {
     lo = hi = make_uint4(0, 0, 0, 0);
-    if (!here || h >= H) return;
+    if (h >= H) return;
     const int w = h >= a.heads[0];
-    const uint4* row = reinterpret_cast<const uint4*>(row_of<const T>(a.x[w], b, s, h - (w ? a.heads[0] : 0)));
+    const uint4* row = reinterpret_cast<const uint4*>(row_of<const T>(a.x[w], p.b, p.s, h - (w ? a.heads[0] : 0)));
     if (l.has0) lo = row[l.v0];
     if (l.has1) hi = row[l.v1];
   };
+  int unit = blockIdx.x * kWarps + (threadIdx.x >> 5);
+  if (unit >= units) return;
+  Place p = place(unit);
   uint4 lo, hi;
-  load(first, lo, hi);
-
-  const int n_angles = min(1 << a.log_tokens, a.tokens - token0) * half_r;
-  for (int i = threadIdx.x; i < n_angles; i += kThreads) {
-    const int t = i / half_r;
-    table[i] = turn_of(a, token0 + t, i - t * half_r);
-  }
-  __syncthreads();
-  float c[E], sn[E];
-  if (here) lane_turns<E>(a, l, table + local * half_r, c, sn);
-
-  float g[2 * E];
-  int which = -1;
-  const float inv_d = 1.f / a.D;
-  for (int it = 0; it < iters; ++it) {
-    const int h = first + it * step;
-    const int w = h >= a.heads[0];
-    uint4 next_lo, next_hi;
-    load(h + step, next_lo, next_hi);
-    float v[2 * E];
-    Vec<T>::unpack(lo, v);
-    Vec<T>::unpack(hi, v + E);
-    if (kNorm) {
-      if (w != which) {
+  load(p, p.first, lo, hi);
+  double pos = a.r > 0 ? position_at(a, p.b, p.s) : 0.0;
+  for (; unit < units; unit += warps) {
+    __syncwarp();                                  // the previous token's angles are no longer read
+    for (int f = threadIdx.x & 31; f < a.r / 2; f += 32) table[f] = turn_of(a, pos, f);
+    __syncwarp();
+    Place next = p;
+    const bool more = unit + warps < units;
+    if (more) {
+      next = place(unit + warps);
+      if (a.r > 0) pos = position_at(a, next.b, next.s);
+    }
+    Turn<E> t;
+    int which = -1;
+    for (int it = 0; it < iters; ++it) {
+      const int h = p.first + it * step;
+      const int w = h >= a.heads[0];
+      float2 v[E];
+      Vec<T>::unpack(lo, reinterpret_cast<float*>(v));
+      Vec<T>::unpack(hi, reinterpret_cast<float*>(v + E / 2));
+      if (it + 1 < iters) load(p, h + step, lo, hi);
+      else if (more) load(next, next.first, lo, hi);
+      if (kNorm ? w != which : which < 0) {
         which = w;
-#pragma unroll
-        for (int e = 0; e < E; ++e) {
-          g[e] = l.has0 ? load_gamma(a, w, l.v0 * E + e) : 0.f;
-          g[E + e] = l.has1 ? load_gamma(a, w, l.v1 * E + e) : 0.f;
-        }
+        lane_turn<E, kInter, kNorm>(a, l, table, smem + w * a.D, t);
       }
-      float ss = 0.f;
+      if (kNorm) {
+        float2 ss = make_float2(0.f, 0.f);
 #pragma unroll
-      for (int e = 0; e < 2 * E; ++e) ss = fmaf(v[e], v[e], ss);
-      const float rstd = 1.f / sqrtf(group_sum(ss, a.log_lanes) * inv_d + a.eps);
+        for (int e = 0; e < E; ++e) ss = __ffma2_rn(v[e], v[e], ss);
+        const float rstd = rsqrtf(group_sum(ss.x + ss.y, a.log_lanes) * inv_d + a.eps);
 #pragma unroll
-      for (int e = 0; e < 2 * E; ++e) v[e] = v[e] * rstd * g[e];
+        for (int e = 0; e < E; ++e) v[e] = __fmul2_rn(v[e], make_float2(rstd, rstd));
+      }
+      if (h < H) {
+        apply<E, kInter>(a, l, t, v);
+        uint4* row = reinterpret_cast<uint4*>(row_of<T>(a.y[w], p.b, p.s, h - (w ? a.heads[0] : 0)));
+        if (l.has0) row[l.v0] = Vec<T>::pack(reinterpret_cast<float*>(v));
+        if (l.has1) row[l.v1] = Vec<T>::pack(reinterpret_cast<float*>(v + E / 2));
+      }
     }
-    if (here && h < H) {
-      rotate<E, kInter>(a, l, c, sn, v, false);
-      uint4* row = reinterpret_cast<uint4*>(row_of<T>(a.y[w], b, s, h - (w ? a.heads[0] : 0)));
-      if (l.has0) row[l.v0] = Vec<T>::pack(v);
-      if (l.has1) row[l.v1] = Vec<T>::pack(v + E);
-    }
-    lo = next_lo, hi = next_hi;
+    p = next;
   }
 }
 
 // --------------------------------------------------------------------------------------------------------------
 // Backward through norm and rotation, whole 16-byte vectors.  Each CTA owns queries or keys (so that one set of dgamma
-// sums stays in registers) and strides over the token chunks.
+// sums stays in registers); its warps stride over the tokens like the forward's.
 // --------------------------------------------------------------------------------------------------------------
 template <typename T, bool kInter>
-__global__ void __launch_bounds__(kThreads) rotary_bwd_kernel(const RotaryArgs a) {
+__global__ void __launch_bounds__(kThreads, 2) rotary_bwd_kernel(const RotaryArgs a) {
   constexpr int E = Vec<T>::E;
-  extern __shared__ float2 table[];
-  __shared__ float sums[kThreads * 2 * E];       // [group][lane][2 E]
-  const int half_r = a.r / 2;
-  const int lane = threadIdx.x & ((1 << a.log_lanes) - 1), group = threadIdx.x >> a.log_lanes;
-  const int groups = kThreads >> a.log_lanes;
-  const int per_token = groups >> a.log_tokens;
-  const int local = group / per_token;
+  extern __shared__ float smem[];
+  __shared__ float sums[kThreads * 2 * E];       // [group of the CTA][lane][2 E]
+  float2* table = stage(a, smem);
+  const int lane = threadIdx.x & ((1 << a.log_lanes) - 1), group = (threadIdx.x & 31) >> a.log_lanes;
+  const int groups = 32 >> a.log_lanes;
   const int w = blockIdx.x >= a.q_ctas;
-  const int cta = w ? blockIdx.x - a.q_ctas : blockIdx.x;
-  const int ctas = w ? gridDim.x - a.q_ctas : a.q_ctas;
+  const int warps = (w ? gridDim.x - a.q_ctas : a.q_ctas) * kWarps;
   const int H = a.heads[w];
-  const int first = group - local * per_token;
-  const int iters = (H + per_token - 1) / per_token;
-  const int chunks = (a.tokens + (1 << a.log_tokens) - 1) >> a.log_tokens;
+  const int step = groups * a.slices;
+  const int iters = (H + step - 1) / step;
+  const int units = a.tokens * a.slices;
   const LaneVectors<E> l(a, lane);
   const Operand X = a.x[w], DY = a.dy[w], DX = a.y[w];
   const float inv_d = 1.f / a.D;
+  const float* gamma = smem + w * a.D;
 
-  float g[2 * E], dg[2 * E];
+  float2 g[E], dg[E];
 #pragma unroll
   for (int e = 0; e < E; ++e) {
-    g[e] = l.has0 ? load_gamma(a, w, l.v0 * E + e) : 0.f;
-    g[E + e] = l.has1 ? load_gamma(a, w, l.v1 * E + e) : 0.f;
-    dg[e] = dg[E + e] = 0.f;
+    at(g, e) = l.has0 ? gamma[l.v0 * E + e] : 0.f;
+    at(g, E + e) = l.has1 ? gamma[l.v1 * E + e] : 0.f;
+    dg[e] = make_float2(0.f, 0.f);
   }
-  for (int chunk = cta; chunk < chunks; chunk += ctas) {
-    const int token0 = chunk << a.log_tokens;
-    const int token = token0 + local;
-    const bool here = token < a.tokens;
+  for (int unit = (blockIdx.x - (w ? a.q_ctas : 0)) * kWarps + (threadIdx.x >> 5); unit < units; unit += warps) {
+    const int token = unit / a.slices;
     const int b = token / a.S, s = token - b * a.S;
+    const int first = (unit - token * a.slices) * groups + group;
     auto load = [&](int h, uint4 (&x)[2], uint4 (&y)[2]) {
       x[0] = x[1] = y[0] = y[1] = make_uint4(0, 0, 0, 0);
-      if (!here || h >= H) return;
+      if (h >= H) return;
       const uint4* xr = reinterpret_cast<const uint4*>(row_of<const T>(X, b, s, h));
       const uint4* yr = reinterpret_cast<const uint4*>(row_of<const T>(DY, b, s, h));
       if (l.has0) x[0] = xr[l.v0], y[0] = yr[l.v0];
@@ -342,57 +388,75 @@ __global__ void __launch_bounds__(kThreads) rotary_bwd_kernel(const RotaryArgs a
     };
     uint4 x[2], y[2];
     load(first, x, y);
-    __syncthreads();                             // the previous chunk's angles are no longer read
-    const int n_angles = min(1 << a.log_tokens, a.tokens - token0) * half_r;
-    for (int i = threadIdx.x; i < n_angles; i += kThreads) {
-      const int t = i / half_r;
-      table[i] = turn_of(a, token0 + t, i - t * half_r);
+    const double pos = a.r > 0 ? position_at(a, b, s) : 0.0;
+    __syncwarp();
+    for (int f = threadIdx.x & 31; f < a.r / 2; f += 32) table[f] = turn_of(a, pos, f);
+    __syncwarp();
+    float2 c[E / 2], sn[E / 2];
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      const int f = angle_of<E, kInter>(a, l, e);
+      const float2 cs = f < a.r / 2 ? table[f] : make_float2(1.f, 0.f);
+      at(c, e) = cs.x, at(sn, e) = cs.y;
     }
-    __syncthreads();
-    float c[E], sn[E];
-    if (here) lane_turns<E>(a, l, table + local * half_r, c, sn);
     for (int it = 0; it < iters; ++it) {
-      const int h = first + it * per_token;
-      const bool on = here && h < H;
-      float v[2 * E], d[2 * E];
-      Vec<T>::unpack(x[0], v);
-      Vec<T>::unpack(x[1], v + E);
-      Vec<T>::unpack(y[0], d);
-      Vec<T>::unpack(y[1], d + E);
-      load(h + per_token, x, y);
-      if (on) rotate<E, kInter>(a, l, c, sn, d, true);
-      float ss = 0.f, xt = 0.f;
+      const int h = first + it * step;
+      float2 v[E], d[E];
+      Vec<T>::unpack(x[0], reinterpret_cast<float*>(v));
+      Vec<T>::unpack(x[1], reinterpret_cast<float*>(v + E / 2));
+      Vec<T>::unpack(y[0], reinterpret_cast<float*>(d));
+      Vec<T>::unpack(y[1], reinterpret_cast<float*>(d + E / 2));
+      if (it + 1 < iters) load(h + step, x, y);
+      // d = R^T dy
+      if (kInter) {
 #pragma unroll
-      for (int e = 0; e < 2 * E; ++e) {
-        ss = fmaf(v[e], v[e], ss);
-        xt = fmaf(v[e] * g[e], d[e], xt);
+        for (int e = 0; e < E; ++e) {
+          const float2 t = d[e];
+          const float ce = (e & 1) ? c[e / 2].y : c[e / 2].x, se = (e & 1) ? sn[e / 2].y : sn[e / 2].x;
+          if (angle_of<E, kInter>(a, l, e) < a.r / 2)
+            d[e] = make_float2(fmaf(t.y, se, t.x * ce), fmaf(-t.x, se, t.y * ce));
+        }
+      } else if (l.turns) {
+#pragma unroll
+        for (int e = 0; e < E / 2; ++e) {
+          const float2 p = d[e], q = d[E / 2 + e];
+          d[e] = __ffma2_rn(q, sn[e], __fmul2_rn(p, c[e]));
+          d[E / 2 + e] = __ffma2_rn(p, make_float2(-sn[e].x, -sn[e].y), __fmul2_rn(q, c[e]));
+        }
       }
-      ss = group_sum(ss, a.log_lanes);
-      xt = group_sum(xt, a.log_lanes);
-      const float rstd = 1.f / sqrtf(ss * inv_d + a.eps);
-      const float k = rstd * rstd * rstd * xt * inv_d;
-      if (on) {
+      float2 ss = make_float2(0.f, 0.f), xt = make_float2(0.f, 0.f);
 #pragma unroll
-        for (int e = 0; e < 2 * E; ++e) {
-          dg[e] = fmaf(v[e] * rstd, d[e], dg[e]);
-          d[e] = rstd * (g[e] * d[e]) - v[e] * k;
+      for (int e = 0; e < E; ++e) {
+        ss = __ffma2_rn(v[e], v[e], ss);
+        xt = __ffma2_rn(__fmul2_rn(v[e], g[e]), d[e], xt);
+      }
+      const float total = group_sum(ss.x + ss.y, a.log_lanes), along = group_sum(xt.x + xt.y, a.log_lanes);
+      const float rstd = rsqrtf(total * inv_d + a.eps);
+      const float k = -rstd * rstd * rstd * along * inv_d;
+      if (h < H) {
+        const float2 r2 = make_float2(rstd, rstd), k2 = make_float2(k, k);
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+          const float2 rd = __fmul2_rn(r2, d[e]);
+          dg[e] = __ffma2_rn(v[e], rd, dg[e]);
+          d[e] = __ffma2_rn(v[e], k2, __fmul2_rn(g[e], rd));
         }
         uint4* row = reinterpret_cast<uint4*>(row_of<T>(DX, b, s, h));
-        if (l.has0) row[l.v0] = Vec<T>::pack(d);
-        if (l.has1) row[l.v1] = Vec<T>::pack(d + E);
+        if (l.has0) row[l.v0] = Vec<T>::pack(reinterpret_cast<float*>(d));
+        if (l.has1) row[l.v1] = Vec<T>::pack(reinterpret_cast<float*>(d + E / 2));
       }
     }
   }
   if (a.partial == nullptr) return;
   // sums of this CTA in group order, then one row of partial sums per CTA: the same order in every run
 #pragma unroll
-  for (int e = 0; e < 2 * E; ++e) sums[threadIdx.x * 2 * E + e] = dg[e];
+  for (int e = 0; e < 2 * E; ++e) sums[threadIdx.x * 2 * E + e] = at(dg, e);
   __syncthreads();
-  if (group == 0) {
+  if (threadIdx.x < (1 << a.log_lanes)) {
 #pragma unroll
     for (int e = 0; e < 2 * E; ++e) {
       float t = 0.f;
-      for (int k = 0; k < groups; ++k) t += sums[((k << a.log_lanes) + lane) * 2 * E + e];
+      for (int k = 0; k < kThreads >> a.log_lanes; ++k) t += sums[((k << a.log_lanes) + lane) * 2 * E + e];
       const int v = e < E ? l.v0 : l.v1;
       if (e < E ? l.has0 : l.has1) a.partial[static_cast<int64_t>(blockIdx.x) * a.D + v * E + (e & (E - 1))] = t;
     }
@@ -417,9 +481,9 @@ __global__ void __launch_bounds__(kThreads) rotary_any_kernel(const RotaryArgs a
     for (int i = lane; i < a.D; i += 32) dg[i] = 0.f;
   for (int token = cta; token < a.tokens; token += ctas) {
     __syncthreads();
-    for (int i = threadIdx.x; i < half_r; i += kThreads) table[i] = turn_of(a, token, i);
-    __syncthreads();
     const int b = token / a.S, s = token - b * a.S;
+    for (int i = threadIdx.x; i < half_r; i += kThreads) table[i] = turn_of(a, position_at(a, b, s), i);
+    __syncthreads();
     for (int hh = warp; hh < H; hh += kWarps) {
       const int w = kBwd ? w0 : hh >= a.heads[0];
       const int h = !kBwd && w ? hh - a.heads[0] : hh;
@@ -602,6 +666,19 @@ int log2_of(int64_t v) {
   return l;
 }
 
+// Parts of a token's heads: one, unless the tokens are fewer than four for each warp that can be resident (a second
+// part costs the token's angles once more, an idle warp more than that).  No part has less than one row for a group.
+int32_t slices_for(int64_t tokens, int64_t heads, int64_t groups, int64_t warps) {
+  const int64_t most = (heads + groups - 1) / groups;
+  int64_t slices = (4 * warps + tokens - 1) / tokens;
+  if (slices > most) slices = most;
+  return static_cast<int32_t>(slices < 1 ? 1 : slices);
+}
+
+size_t vector_smem(const RotaryArgs& a) {
+  return (a.norm ? 2 * a.D * sizeof(float) : 0) + static_cast<size_t>(kWarps) * (a.r / 2) * sizeof(float2);
+}
+
 template <typename T>
 int32_t launch_fwd(RotaryArgs a, const Problem& pr, cudaStream_t st) {
   int sms = 0;
@@ -617,22 +694,11 @@ int32_t launch_fwd(RotaryArgs a, const Problem& pr, cudaStream_t st) {
     const int64_t grid = tokens < sms * 8ll ? tokens : sms * 8ll;
     rotary_any_kernel<T, false><<<static_cast<unsigned>(grid), kThreads, a.r / 2 * sizeof(float2), st>>>(a);
   } else {
-    const int groups = kThreads / lanes;
-    // Tokens per CTA: enough rows for every group (about two each), but no fewer CTAs than SMs.
-    int log_t = log2_of(groups);
-    while (log_t > 0 && ((tokens + (1 << log_t) - 1) >> log_t) < 4ll * sms) --log_t;
-    while (log_t > 0 && (groups >> log_t) < 2 && H > 4) --log_t;
     a.log_lanes = log2_of(lanes);
-    a.log_tokens = log_t;
-    const int per_token = groups >> log_t;
-    // one token per CTA: its heads are spread over more CTAs when few tokens would leave SMs idle
-    int64_t y = 1;
-    if (log_t == 0) {
-      y = (H + per_token - 1) / per_token;
-      if (tokens * y > 2ll * sms) y = 1;
-    }
-    const dim3 grid(static_cast<unsigned>((tokens + (1 << log_t) - 1) >> log_t), static_cast<unsigned>(y));
-    const size_t smem = (size_t{1} << log_t) * (a.r / 2) * sizeof(float2);
+    a.slices = slices_for(tokens, H, 32 / lanes, 16ll * sms);
+    const int64_t units = tokens * a.slices, most = 2ll * sms;
+    const unsigned grid = static_cast<unsigned>(units < most * kWarps ? (units + kWarps - 1) / kWarps : most);
+    const size_t smem = vector_smem(a);
     if (a.norm) {
       if (a.interleaved) rotary_fwd_kernel<T, true, true><<<grid, kThreads, smem, st>>>(a);
       else rotary_fwd_kernel<T, true, false><<<grid, kThreads, smem, st>>>(a);
@@ -656,23 +722,21 @@ int32_t launch_bwd(RotaryArgs a, const Problem& pr, float* dq_gamma, float* dk_g
   for (int w = 0; w < 2; ++w)
     if (pr.H[w] > 0 && !(is_vector_operand(a.x[w], E) && is_vector_operand(a.y[w], E) && is_vector_operand(a.dy[w], E)))
       lanes = 0;
-  int log_t = 0;
-  if (lanes != 0) {
-    const int groups = kThreads / lanes;
-    log_t = log2_of(groups);
-    while (log_t > 0 && ((static_cast<int64_t>(a.tokens) + (1 << log_t) - 1) >> log_t) < 4ll * sms) --log_t;
-    while (log_t > 0 && (groups >> log_t) < 2 && a.heads[0] > 4) --log_t;
-    a.log_lanes = log2_of(lanes);
-    a.log_tokens = log_t;
-  }
   // CTAs of queries and of keys in the ratio of their heads, at least one each where there are heads
-  const int64_t chunks = (static_cast<int64_t>(a.tokens) + (1 << log_t) - 1) >> log_t;
   const int64_t slots = 2ll * sms, H = pr.H[0] + pr.H[1];
+  int64_t per_cta = 1;
+  if (lanes != 0) {
+    a.log_lanes = log2_of(lanes);
+    a.slices = slices_for(a.tokens, a.heads[0] > a.heads[1] ? a.heads[0] : a.heads[1], 32 / lanes, 16ll * sms);
+    per_cta = kWarps;
+  }
+  const int64_t units = static_cast<int64_t>(a.tokens) * (lanes != 0 ? a.slices : 1);
   int64_t ctas[2];
   for (int w = 0; w < 2; ++w) {
     ctas[w] = slots * pr.H[w] / H;
     if (ctas[w] == 0 && pr.H[w] > 0) ctas[w] = 1;
-    if (ctas[w] > chunks) ctas[w] = chunks;
+    const int64_t most = (units + per_cta - 1) / per_cta;
+    if (ctas[w] > most) ctas[w] = most;
   }
   a.q_ctas = static_cast<int32_t>(ctas[0]);
   const int64_t grid = ctas[0] + ctas[1];
@@ -685,7 +749,7 @@ int32_t launch_bwd(RotaryArgs a, const Problem& pr, float* dq_gamma, float* dk_g
     const size_t smem = a.r / 2 * sizeof(float2) + static_cast<size_t>(kWarps) * a.D * sizeof(float);
     rotary_any_kernel<T, true><<<static_cast<unsigned>(grid), kThreads, smem, st>>>(a);
   } else {
-    const size_t smem = (size_t{1} << log_t) * (a.r / 2) * sizeof(float2);
+    const size_t smem = vector_smem(a);
     if (a.interleaved) rotary_bwd_kernel<T, true><<<static_cast<unsigned>(grid), kThreads, smem, st>>>(a);
     else rotary_bwd_kernel<T, false><<<static_cast<unsigned>(grid), kThreads, smem, st>>>(a);
   }
