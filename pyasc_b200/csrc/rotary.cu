@@ -42,7 +42,7 @@ struct RotaryArgs {
   int32_t D, r;
   int32_t log_lanes;       // lanes per row (vector kernels)
   int32_t slices;          // parts a token's heads are cut into, one warp each (vector kernels)
-  int32_t q_ctas;          // backward: CTAs [0, q_ctas) own queries, the others keys
+  int32_t q_ctas;          // any-size backward: CTAs [0, q_ctas) own queries, the others keys
   int32_t gamma_type;      // 0 fp16, 1 bf16, 2 fp32
   int32_t pos32;           // positions are int32 instead of int64
   int32_t norm, interleaved, conj;
@@ -345,120 +345,158 @@ __global__ void __launch_bounds__(kThreads) rotary_fwd_kernel(const RotaryArgs a
 }
 
 // --------------------------------------------------------------------------------------------------------------
-// Backward through norm and rotation, whole 16-byte vectors.  Each CTA owns queries or keys (so that one set of dgamma
-// sums stays in registers); its warps stride over the tokens like the forward's.
+// Backward through norm and rotation, whole 16-byte vectors: the forward's division of the work.  A lane's sums for
+// dgamma stay in registers over a token's queries (then its keys) and are added to the lane's own place in shared memory
+// after them, so that queries and keys share the angles without two sets of sums in registers.
 // --------------------------------------------------------------------------------------------------------------
 template <typename T, bool kInter>
 __global__ void __launch_bounds__(kThreads, 2) rotary_bwd_kernel(const RotaryArgs a) {
   constexpr int E = Vec<T>::E;
   extern __shared__ float smem[];
-  __shared__ float sums[kThreads * 2 * E];       // [group of the CTA][lane][2 E]
   float2* table = stage(a, smem);
+  // [queries, keys][pair][thread], behind the angles
+  float2* sums = reinterpret_cast<float2*>(smem + 2 * a.D) + kWarps * (a.r / 2);
   const int lane = threadIdx.x & ((1 << a.log_lanes) - 1), group = (threadIdx.x & 31) >> a.log_lanes;
   const int groups = 32 >> a.log_lanes;
-  const int w = blockIdx.x >= a.q_ctas;
-  const int warps = (w ? gridDim.x - a.q_ctas : a.q_ctas) * kWarps;
-  const int H = a.heads[w];
+  const int H = a.heads[0] + a.heads[1];
   const int step = groups * a.slices;
   const int iters = (H + step - 1) / step;
+  const int warps = gridDim.x * kWarps;
   const int units = a.tokens * a.slices;
   const LaneVectors<E> l(a, lane);
-  const Operand X = a.x[w], DY = a.dy[w], DX = a.y[w];
   const float inv_d = 1.f / a.D;
-  const float* gamma = smem + w * a.D;
+#pragma unroll
+  for (int e = 0; e < 2 * E; ++e) sums[e * kThreads + threadIdx.x] = make_float2(0.f, 0.f);
 
-  float2 g[E], dg[E];
-#pragma unroll
-  for (int e = 0; e < E; ++e) {
-    at(g, e) = l.has0 ? gamma[l.v0 * E + e] : 0.f;
-    at(g, E + e) = l.has1 ? gamma[l.v1 * E + e] : 0.f;
-    dg[e] = make_float2(0.f, 0.f);
-  }
-  for (int unit = (blockIdx.x - (w ? a.q_ctas : 0)) * kWarps + (threadIdx.x >> 5); unit < units; unit += warps) {
+  struct Place {
+    int b, s, first;
+  };
+  auto place = [&](int unit) {
     const int token = unit / a.slices;
-    const int b = token / a.S, s = token - b * a.S;
-    const int first = (unit - token * a.slices) * groups + group;
-    auto load = [&](int h, uint4 (&x)[2], uint4 (&y)[2]) {
-      x[0] = x[1] = y[0] = y[1] = make_uint4(0, 0, 0, 0);
-      if (h >= H) return;
-      const uint4* xr = reinterpret_cast<const uint4*>(row_of<const T>(X, b, s, h));
-      const uint4* yr = reinterpret_cast<const uint4*>(row_of<const T>(DY, b, s, h));
-      if (l.has0) x[0] = xr[l.v0], y[0] = yr[l.v0];
-      if (l.has1) x[1] = xr[l.v1], y[1] = yr[l.v1];
-    };
+    const int b = token / a.S;
+    return Place{b, token - b * a.S, (unit - token * a.slices) * groups + group};
+  };
+  auto load = [&](const Place& p, int h, uint4 (&x)[2], uint4 (&y)[2]) {
+    x[0] = x[1] = y[0] = y[1] = make_uint4(0, 0, 0, 0);
+    if (h >= H) return;
+    const int w = h >= a.heads[0];
+    const int hw = h - (w ? a.heads[0] : 0);
+    const uint4* xr = reinterpret_cast<const uint4*>(row_of<const T>(a.x[w], p.b, p.s, hw));
+    const uint4* yr = reinterpret_cast<const uint4*>(row_of<const T>(a.dy[w], p.b, p.s, hw));
+    if (l.has0) x[0] = xr[l.v0], y[0] = yr[l.v0];
+    if (l.has1) x[1] = xr[l.v1], y[1] = yr[l.v1];
+  };
+  float2 g[E], dg[E];
+  int which = -1;
+  auto flush = [&]() {
+    float2* to = sums + which * E * kThreads + threadIdx.x;
+#pragma unroll
+    for (int e = 0; e < E; ++e) to[e * kThreads] = __fadd2_rn(to[e * kThreads], dg[e]);
+  };
+  int unit = blockIdx.x * kWarps + (threadIdx.x >> 5);
+  if (unit < units) {
+    Place p = place(unit);
     uint4 x[2], y[2];
-    load(first, x, y);
-    const double pos = a.r > 0 ? position_at(a, b, s) : 0.0;
-    __syncwarp();
-    for (int f = threadIdx.x & 31; f < a.r / 2; f += 32) table[f] = turn_of(a, pos, f);
-    __syncwarp();
-    float2 c[E / 2], sn[E / 2];
-#pragma unroll
-    for (int e = 0; e < E; ++e) {
-      const int f = angle_of<E, kInter>(a, l, e);
-      const float2 cs = f < a.r / 2 ? table[f] : make_float2(1.f, 0.f);
-      at(c, e) = cs.x, at(sn, e) = cs.y;
-    }
-    for (int it = 0; it < iters; ++it) {
-      const int h = first + it * step;
-      float2 v[E], d[E];
-      Vec<T>::unpack(x[0], reinterpret_cast<float*>(v));
-      Vec<T>::unpack(x[1], reinterpret_cast<float*>(v + E / 2));
-      Vec<T>::unpack(y[0], reinterpret_cast<float*>(d));
-      Vec<T>::unpack(y[1], reinterpret_cast<float*>(d + E / 2));
-      if (it + 1 < iters) load(h + step, x, y);
-      // d = R^T dy
-      if (kInter) {
-#pragma unroll
-        for (int e = 0; e < E; ++e) {
-          const float2 t = d[e];
-          const float ce = (e & 1) ? c[e / 2].y : c[e / 2].x, se = (e & 1) ? sn[e / 2].y : sn[e / 2].x;
-          if (angle_of<E, kInter>(a, l, e) < a.r / 2)
-            d[e] = make_float2(fmaf(t.y, se, t.x * ce), fmaf(-t.x, se, t.y * ce));
-        }
-      } else if (l.turns) {
-#pragma unroll
-        for (int e = 0; e < E / 2; ++e) {
-          const float2 p = d[e], q = d[E / 2 + e];
-          d[e] = __ffma2_rn(q, sn[e], __fmul2_rn(p, c[e]));
-          d[E / 2 + e] = __ffma2_rn(p, make_float2(-sn[e].x, -sn[e].y), __fmul2_rn(q, c[e]));
-        }
+    load(p, p.first, x, y);
+    double pos = a.r > 0 ? position_at(a, p.b, p.s) : 0.0;
+    for (; unit < units; unit += warps) {
+      __syncwarp();
+      for (int f = threadIdx.x & 31; f < a.r / 2; f += 32) table[f] = turn_of(a, pos, f);
+      __syncwarp();
+      Place next = p;
+      const bool more = unit + warps < units;
+      if (more) {
+        next = place(unit + warps);
+        if (a.r > 0) pos = position_at(a, next.b, next.s);
       }
-      float2 ss = make_float2(0.f, 0.f), xt = make_float2(0.f, 0.f);
+      float2 c[E / 2], sn[E / 2];
 #pragma unroll
       for (int e = 0; e < E; ++e) {
-        ss = __ffma2_rn(v[e], v[e], ss);
-        xt = __ffma2_rn(__fmul2_rn(v[e], g[e]), d[e], xt);
+        const int f = angle_of<E, kInter>(a, l, e);
+        const float2 cs = f < a.r / 2 ? table[f] : make_float2(1.f, 0.f);
+        at(c, e) = cs.x, at(sn, e) = cs.y;
       }
-      const float total = group_sum(ss.x + ss.y, a.log_lanes), along = group_sum(xt.x + xt.y, a.log_lanes);
-      const float rstd = rsqrtf(total * inv_d + a.eps);
-      const float k = -rstd * rstd * rstd * along * inv_d;
-      if (h < H) {
-        const float2 r2 = make_float2(rstd, rstd), k2 = make_float2(k, k);
+      for (int it = 0; it < iters; ++it) {
+        const int h = p.first + it * step;
+        const int w = h >= a.heads[0];
+        if (w != which) {
+          if (which >= 0) flush();
+          which = w;
+          const float* gamma = smem + w * a.D;
+#pragma unroll
+          for (int e = 0; e < E; ++e) {
+            at(g, e) = l.has0 ? gamma[l.v0 * E + e] : 0.f;
+            at(g, E + e) = l.has1 ? gamma[l.v1 * E + e] : 0.f;
+            dg[e] = make_float2(0.f, 0.f);
+          }
+        }
+        float2 v[E], d[E];
+        Vec<T>::unpack(x[0], reinterpret_cast<float*>(v));
+        Vec<T>::unpack(x[1], reinterpret_cast<float*>(v + E / 2));
+        Vec<T>::unpack(y[0], reinterpret_cast<float*>(d));
+        Vec<T>::unpack(y[1], reinterpret_cast<float*>(d + E / 2));
+        if (it + 1 < iters) load(p, h + step, x, y);
+        else if (more) load(next, next.first, x, y);
+        // d = R^T dy
+        if (kInter) {
+#pragma unroll
+          for (int e = 0; e < E; ++e) {
+            const float2 t = d[e];
+            const float ce = (e & 1) ? c[e / 2].y : c[e / 2].x, se = (e & 1) ? sn[e / 2].y : sn[e / 2].x;
+            if (angle_of<E, kInter>(a, l, e) < a.r / 2)
+              d[e] = make_float2(fmaf(t.y, se, t.x * ce), fmaf(-t.x, se, t.y * ce));
+          }
+        } else if (l.turns) {
+#pragma unroll
+          for (int e = 0; e < E / 2; ++e) {
+            const float2 q = d[e], r = d[E / 2 + e];
+            d[e] = __ffma2_rn(r, sn[e], __fmul2_rn(q, c[e]));
+            d[E / 2 + e] = __ffma2_rn(q, make_float2(-sn[e].x, -sn[e].y), __fmul2_rn(r, c[e]));
+          }
+        }
+        float2 ss = make_float2(0.f, 0.f), xt = make_float2(0.f, 0.f);
 #pragma unroll
         for (int e = 0; e < E; ++e) {
-          const float2 rd = __fmul2_rn(r2, d[e]);
-          dg[e] = __ffma2_rn(v[e], rd, dg[e]);
-          d[e] = __ffma2_rn(v[e], k2, __fmul2_rn(g[e], rd));
+          ss = __ffma2_rn(v[e], v[e], ss);
+          xt = __ffma2_rn(__fmul2_rn(v[e], g[e]), d[e], xt);
         }
-        uint4* row = reinterpret_cast<uint4*>(row_of<T>(DX, b, s, h));
-        if (l.has0) row[l.v0] = Vec<T>::pack(reinterpret_cast<float*>(d));
-        if (l.has1) row[l.v1] = Vec<T>::pack(reinterpret_cast<float*>(d + E / 2));
+        const float total = group_sum(ss.x + ss.y, a.log_lanes), along = group_sum(xt.x + xt.y, a.log_lanes);
+        const float rstd = rsqrtf(total * inv_d + a.eps);
+        const float k = -rstd * rstd * rstd * along * inv_d;
+        if (h < H) {
+          const float2 r2 = make_float2(rstd, rstd), k2 = make_float2(k, k);
+#pragma unroll
+          for (int e = 0; e < E; ++e) {
+            const float2 rd = __fmul2_rn(r2, d[e]);
+            dg[e] = __ffma2_rn(v[e], rd, dg[e]);
+            d[e] = __ffma2_rn(v[e], k2, __fmul2_rn(g[e], rd));
+          }
+          uint4* row = reinterpret_cast<uint4*>(row_of<T>(a.y[w], p.b, p.s, h - (w ? a.heads[0] : 0)));
+          if (l.has0) row[l.v0] = Vec<T>::pack(reinterpret_cast<float*>(d));
+          if (l.has1) row[l.v1] = Vec<T>::pack(reinterpret_cast<float*>(d + E / 2));
+        }
       }
+      p = next;
     }
+    flush();
   }
   if (a.partial == nullptr) return;
-  // sums of this CTA in group order, then one row of partial sums per CTA: the same order in every run
-#pragma unroll
-  for (int e = 0; e < 2 * E; ++e) sums[threadIdx.x * 2 * E + e] = at(dg, e);
+  // sums of this CTA in group order, then one row of partial sums of queries and one of keys per CTA: the same order in
+  // every run
   __syncthreads();
-  if (threadIdx.x < (1 << a.log_lanes)) {
-#pragma unroll
-    for (int e = 0; e < 2 * E; ++e) {
-      float t = 0.f;
-      for (int k = 0; k < kThreads >> a.log_lanes; ++k) t += sums[((k << a.log_lanes) + lane) * 2 * E + e];
-      const int v = e < E ? l.v0 : l.v1;
-      if (e < E ? l.has0 : l.has1) a.partial[static_cast<int64_t>(blockIdx.x) * a.D + v * E + (e & (E - 1))] = t;
+  const int per_row = 1 << a.log_lanes;
+  for (int i = threadIdx.x; i < 2 * E * per_row; i += kThreads) {
+    const int e = i >> a.log_lanes, at_lane = i & (per_row - 1);       // e < E: queries
+    float2 t = make_float2(0.f, 0.f);
+    for (int k = 0; k < kThreads >> a.log_lanes; ++k)
+      t = __fadd2_rn(t, sums[e * kThreads + (k << a.log_lanes) + at_lane]);
+    const LaneVectors<E> o(a, at_lane);
+    const int pair = e & (E - 1);
+    const bool lo = pair < E / 2;
+    if (lo ? o.has0 : o.has1) {
+      float* to = a.partial + (static_cast<int64_t>(e >= E ? gridDim.x : 0) + blockIdx.x) * a.D +
+                  (lo ? o.v0 : o.v1) * E + 2 * (pair & (E / 2 - 1));
+      to[0] = t.x, to[1] = t.y;
     }
   }
 }
@@ -564,12 +602,13 @@ __global__ void __launch_bounds__(kThreads) rotary_any_kernel(const RotaryArgs a
   }
 }
 
-// dgamma[w][c] = sum over the CTAs of queries (w = 0) or keys (w = 1), in a fixed order: 8 interleaved sums in 64 bits
-__global__ void __launch_bounds__(256) dgamma_kernel(const float* partial, int q_ctas, int ctas, int D, float* dq_gamma,
+// dgamma[w][c] = sum over the rows of partial sums of queries (w = 0; the first q_rows) or keys (w = 1), in a fixed
+// order: 8 interleaved sums in 64 bits
+__global__ void __launch_bounds__(256) dgamma_kernel(const float* partial, int q_rows, int rows, int D, float* dq_gamma,
                                                      float* dk_gamma) {
   __shared__ double red[8][32];
   const int c = blockIdx.x * 32 + (threadIdx.x & 31), part = threadIdx.x >> 5;
-  const int lo = blockIdx.y ? q_ctas : 0, hi = blockIdx.y ? ctas : q_ctas;
+  const int lo = blockIdx.y ? q_rows : 0, hi = blockIdx.y ? rows : q_rows;
   float* out = blockIdx.y ? dk_gamma : dq_gamma;
   double t = 0.0;
   if (c < D)
@@ -722,34 +761,34 @@ int32_t launch_bwd(RotaryArgs a, const Problem& pr, float* dq_gamma, float* dk_g
   for (int w = 0; w < 2; ++w)
     if (pr.H[w] > 0 && !(is_vector_operand(a.x[w], E) && is_vector_operand(a.y[w], E) && is_vector_operand(a.dy[w], E)))
       lanes = 0;
-  // CTAs of queries and of keys in the ratio of their heads, at least one each where there are heads
+  const size_t smem = vector_smem(a) + 2 * E * kThreads * sizeof(float2);
+  if (smem > 48 * 1024) lanes = 0;      // 16-bit heads of more than 448: not worth a larger share of the L1 cache
   const int64_t slots = 2ll * sms, H = pr.H[0] + pr.H[1];
-  int64_t per_cta = 1;
+  int64_t rows[2];             // rows of partial sums of the gammas, queries' first
   if (lanes != 0) {
     a.log_lanes = log2_of(lanes);
-    a.slices = slices_for(a.tokens, a.heads[0] > a.heads[1] ? a.heads[0] : a.heads[1], 32 / lanes, 16ll * sms);
-    per_cta = kWarps;
+    a.slices = slices_for(a.tokens, H, 32 / lanes, 8ll * slots);
+    const int64_t units = static_cast<int64_t>(a.tokens) * a.slices;
+    rows[0] = rows[1] = units < slots * kWarps ? (units + kWarps - 1) / kWarps : slots;
+  } else {
+    // CTAs of queries and of keys in the ratio of their heads, at least one each where there are heads
+    for (int w = 0; w < 2; ++w) {
+      rows[w] = slots * pr.H[w] / H;
+      if (rows[w] == 0 && pr.H[w] > 0) rows[w] = 1;
+      if (rows[w] > a.tokens) rows[w] = a.tokens;
+    }
   }
-  const int64_t units = static_cast<int64_t>(a.tokens) * (lanes != 0 ? a.slices : 1);
-  int64_t ctas[2];
-  for (int w = 0; w < 2; ++w) {
-    ctas[w] = slots * pr.H[w] / H;
-    if (ctas[w] == 0 && pr.H[w] > 0) ctas[w] = 1;
-    const int64_t most = (units + per_cta - 1) / per_cta;
-    if (ctas[w] > most) ctas[w] = most;
-  }
-  a.q_ctas = static_cast<int32_t>(ctas[0]);
-  const int64_t grid = ctas[0] + ctas[1];
+  a.q_ctas = static_cast<int32_t>(rows[0]);
+  const int64_t n_rows = rows[0] + rows[1], grid = lanes != 0 ? rows[0] : n_rows;
   void* ws = nullptr;
   if (dq_gamma != nullptr || dk_gamma != nullptr) {
-    if ((rc = aschost::scratch_alloc(&ws, static_cast<size_t>(grid) * a.D * sizeof(float), st)) != ASC_OK) return rc;
+    if ((rc = aschost::scratch_alloc(&ws, static_cast<size_t>(n_rows) * a.D * sizeof(float), st)) != ASC_OK) return rc;
     a.partial = static_cast<float*>(ws);
   }
   if (lanes == 0) {
-    const size_t smem = a.r / 2 * sizeof(float2) + static_cast<size_t>(kWarps) * a.D * sizeof(float);
-    rotary_any_kernel<T, true><<<static_cast<unsigned>(grid), kThreads, smem, st>>>(a);
+    const size_t any_smem = a.r / 2 * sizeof(float2) + static_cast<size_t>(kWarps) * a.D * sizeof(float);
+    rotary_any_kernel<T, true><<<static_cast<unsigned>(grid), kThreads, any_smem, st>>>(a);
   } else {
-    const size_t smem = vector_smem(a);
     if (a.interleaved) rotary_bwd_kernel<T, true><<<static_cast<unsigned>(grid), kThreads, smem, st>>>(a);
     else rotary_bwd_kernel<T, false><<<static_cast<unsigned>(grid), kThreads, smem, st>>>(a);
   }
@@ -757,7 +796,7 @@ int32_t launch_bwd(RotaryArgs a, const Problem& pr, float* dq_gamma, float* dk_g
   if (e == cudaSuccess) {
     aschost::count_launch();
     if (ws != nullptr) {
-      dgamma_kernel<<<dim3((a.D + 31) / 32, 2), 256, 0, st>>>(a.partial, a.q_ctas, static_cast<int>(grid), a.D, dq_gamma,
+      dgamma_kernel<<<dim3((a.D + 31) / 32, 2), 256, 0, st>>>(a.partial, a.q_ctas, static_cast<int>(n_rows), a.D, dq_gamma,
                                                               dk_gamma);
       e = cudaGetLastError();
       if (e == cudaSuccess) aschost::count_launch();
