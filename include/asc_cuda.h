@@ -342,6 +342,20 @@ int32_t asc_cuda_norm_rotary_bwd(const void* dq_out, const void* dk_out, const v
                                  const int64_t* strides, float eps, float scale, int32_t dtype, int32_t gamma_dtype,
                                  int32_t flags, void* stream);
 
+/* Attention of queries q [B, Sq, Hq, D] to the keys and values k, v [B, Skv, Hkv, D] of another sequence:
+ *   o = softmax(scale * q k^T) v,  lse[b, h, s] = log(sum_t exp(scale * q k^T)) (fp32, contiguous [B, Hq, Sq], or NULL)
+ * Hq is a multiple of Hkv: query head h reads key head h / (Hq / Hkv).  kv_lengths (int32, device, or NULL): keys from
+ * kv_lengths[b] on do not take part, whatever k and v hold there (values outside 0..Skv are clamped); a query without
+ * keys gets o = 0 and lse = -inf.  dims = {B, Sq, Skv, Hq, Hkv, D}, D a multiple of 8 up to 128 (status 3 otherwise).
+ * strides, in elements, the last dimension contiguous: q, k, v, o (three each: batch, sequence, head).  All four 16-byte
+ * aligned with strides in multiples of 8 elements; the batch and head strides of k and v may be 0 (one state for several
+ * entries).  dims and strides are host arrays.  scale >= 0.  dtype: 0 fp16, 1 bf16; fp32 softmax and accumulation, the
+ * probabilities rounded to dtype for the second product.  o must not overlap k or v.  Few rows are cut along the keys
+ * and joined in a fixed order; that workspace is allocated and released on the stream.  No counterpart in the reference. */
+int32_t asc_cuda_cross_attn_fwd_f16(const void* q, const void* k, const void* v, void* o, float* lse,
+                                    const int32_t* kv_lengths, const int64_t* dims, const int64_t* strides, float scale,
+                                    int32_t dtype, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

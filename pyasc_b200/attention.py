@@ -1,5 +1,5 @@
-"""What stands next to the attention of a transformer block, on CUDA torch tensors: rotary positions of queries and
-keys, alone or behind an RMS norm of every head, with their gradients.
+"""What stands next to the self-attention of a transformer block, on CUDA torch tensors: rotary positions of queries and
+keys, alone or behind an RMS norm of every head, and attention to the states of another sequence, with their gradients.
 
 The functions are thin: they check their arguments (``ValueError`` / ``TypeError``), allocate outputs with torch, and
 make one call of the C ABI (``include/asc_cuda.h``) on torch's current stream of the tensors' device.  They return
@@ -72,7 +72,7 @@ def _output(name: str, given: Optional[torch.Tensor], like: torch.Tensor, shape:
     return given
 
 
-_PACK = {n: struct.Struct(f"{n}q").pack for n in (6, 14, 20)}     # host int64 arrays of the C ABI
+_PACK = {n: struct.Struct(f"{n}q").pack for n in (6, 12, 14, 20)}     # host int64 arrays of the C ABI
 _NO_STRIDES = (0, 0, 0)
 
 
@@ -252,3 +252,47 @@ def norm_rotary_backward(dq_out: torch.Tensor, dk_out: Optional[torch.Tensor], q
           _PACK[20](*_strides(dq_out), *_strides(dk_out), *_strides(q), *_strides(k), *_strides(dq), *_strides(dk),
                     *pos_strides), eps, scale, _DTYPE_CODE[q.dtype], gamma_code, 2 | pos_flag | bool(interleaved))
     return dq, dk, dq_gamma, dk_gamma
+
+
+# --------------------------------------------------------------------------------------------------
+# Attention to another sequence
+# --------------------------------------------------------------------------------------------------
+def _cross_arguments(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, kv_lengths: Optional[torch.Tensor],
+                     scale: Optional[float]):
+    device = _device_of("q", q)
+    dtype = q.dtype
+    if dtype not in (torch.float16, torch.bfloat16):
+        raise TypeError(f"q has type {dtype}, expected float16 or bfloat16")
+    q_shape, k_shape = _check_rows("q", q, dtype, device), _check_rows("k", k, dtype, device)
+    batch, seq, heads, head_dim = q_shape
+    kv_seq, kv_heads = k_shape[1], k_shape[2]
+    _check_shape("k", k_shape, (batch, kv_seq, kv_heads, head_dim))
+    _check_shape("v", _check_rows("v", v, dtype, device), k_shape)
+    if heads % kv_heads if kv_heads else heads:
+        raise ValueError(f"{heads} query heads are not a multiple of {kv_heads} key heads")
+    if kv_lengths is not None:
+        _check_vector("kv_lengths", kv_lengths, (torch.int32, ), device)
+        _check_shape("kv_lengths", kv_lengths.shape, (batch, ))
+        if not kv_lengths.is_contiguous():
+            raise ValueError("kv_lengths must be contiguous")
+    if scale is None:
+        scale = head_dim**-0.5 if head_dim else 0.0
+    return device, q_shape, k_shape, _PACK[6](batch, seq, kv_seq, heads, kv_heads, head_dim), scale
+
+
+def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, kv_lengths: Optional[torch.Tensor] = None,
+                    scale: Optional[float] = None, return_lse: bool = False, out: Optional[torch.Tensor] = None):
+    """``softmax(scale q k^T) v`` of queries [B, S, Hq, D] and keys and values [B, T, Hkv, D] of another sequence.
+
+    float16 or bfloat16; D a multiple of 8 up to 128; Hq a multiple of Hkv (grouped heads).  ``kv_lengths`` (int32 [B]):
+    keys from there on do not take part, whatever they hold.  ``scale`` is ``D ** -0.5`` unless given.  k and v may repeat
+    one state (``expand``) over batch or heads.  S = 1 is the form for generated tokens: few rows are cut along the keys
+    and joined.  ``return_lse`` adds the float32 [B, Hq, S] logarithms of the softmax sums, which the gradient needs; a
+    query without keys gives 0 and -inf.  Returns ``out`` or ``(out, lse)``."""
+    device, q_shape, _, dims, scale = _cross_arguments(q, k, v, kv_lengths, scale)
+    out = _output("out", out, q, q_shape, device)
+    lse = torch.empty(q_shape[0], q_shape[2], q_shape[1], dtype=torch.float32, device=q.device) if return_lse else None
+    _call("asc_cuda_cross_attn_fwd_f16", device, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), _ptr(lse),
+          _ptr(kv_lengths), dims, _PACK[12](*_strides(q), *_strides(k), *_strides(v), *_strides(out)), scale,
+          _DTYPE_CODE[q.dtype])
+    return (out, lse) if return_lse else out

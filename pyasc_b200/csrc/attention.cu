@@ -21,6 +21,7 @@
 #include <cuda_bf16.h>
 
 #include "../../include/asc_cuda.h"
+#include "attention_common.cuh"
 #include "host_common.h"
 
 namespace {
@@ -80,28 +81,6 @@ struct AttnCtl {
   uint32_t tmem_base;
   uint32_t abort_flag;
 };
-
-__device__ __forceinline__ float ex2_approx(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-
-__device__ __forceinline__ float max3(float a, float b, float c) {
-  float d;
-  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
-  return d;
-}
-
-template <bool kBf16>
-__device__ __forceinline__ uint32_t pack2(float a, float b) {
-  if (kBf16) {
-    __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
-    return *reinterpret_cast<uint32_t*>(&h);
-  }
-  __half2 h = __floats2half2_rn(a, b);
-  return *reinterpret_cast<uint32_t*>(&h);
-}
 
 // number of key tiles query tile `qt` (128-row index within the head) has to visit
 __device__ __forceinline__ int kv_tiles_for(int qt, int S, int causal) {

@@ -1,0 +1,60 @@
+"""Attention to another sequence without a GPU: status codes of the C ABI and refusals of host tensors."""
+import ctypes
+
+import pytest
+import torch
+
+from pyasc_b200 import attention as A
+from pyasc_b200 import capi
+
+
+def forward(dims, strides=(64, ) * 12, scale=1.0, dtype=0, q_off=0, k_null=False, lse_off=None):
+    buf = (ctypes.c_double * 64)()
+    p = (ctypes.addressof(buf) + 15) // 16 * 16
+    return capi.load().asc_cuda_cross_attn_fwd_f16(p + q_off, None if k_null else p, p, p, None if lse_off is None else p + lse_off,
+                                                   None, (ctypes.c_int64 * 6)(*dims), (ctypes.c_int64 * 12)(*strides), scale,
+                                                   dtype, None)
+
+
+GOOD = (2, 3, 4, 2, 2, 64)
+
+
+def changed(i, value, base=GOOD):
+    return tuple(value if j == i else x for j, x in enumerate(base))
+
+
+def test_nothing_to_do():
+    for i in (0, 1):
+        assert forward(changed(i, 0)) == 0
+    assert forward((2, 3, 4, 0, 0, 64)) == 0
+
+
+def test_status_codes():
+    for i in range(6):
+        assert forward(changed(i, -1)) == 1
+    assert forward((2, 3, 4, 3, 2, 64)) == 1           # heads that do not group
+    assert forward((2, 3, 4, 3, 0, 64)) == 1
+    assert forward(changed(5, 60)) == 3
+    assert forward(changed(5, 136)) == 3
+    assert forward(GOOD, dtype=2) == 1
+    assert forward(GOOD, scale=-0.5) == 1
+    assert forward(GOOD, scale=float("nan")) == 1
+    assert forward(GOOD, scale=float("inf")) == 1
+    assert forward(GOOD, q_off=2) == 2
+    assert forward(GOOD, k_null=True) == 1
+    assert forward(GOOD, lse_off=2) == 2
+    for i in range(12):
+        assert forward(GOOD, strides=changed(i, 60, (64, ) * 12)) == 2
+        assert forward(GOOD, strides=changed(i, -64, (64, ) * 12)) == 1
+    for i in (0, 2, 1, 4, 7, 9, 10, 11):               # a stride of 0 only over batch and heads of k and v
+        assert forward(GOOD, strides=changed(i, 0, (64, ) * 12)) == 1
+    assert forward(GOOD, strides=changed(3, 1 << 39, (64, ) * 12)) == 6
+    assert forward(changed(0, 1 << 25)) == 6
+
+
+def test_host_tensors_are_refused():
+    q = torch.zeros(1, 2, 2, 64, dtype=torch.float16)
+    with pytest.raises(ValueError, match="CUDA"):
+        A.cross_attention(q, q, q)
+    with pytest.raises(TypeError):
+        A.cross_attention(None, q, q)
