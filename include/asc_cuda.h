@@ -355,6 +355,16 @@ int32_t asc_cuda_norm_rotary_bwd(const void* dq_out, const void* dk_out, const v
 int32_t asc_cuda_cross_attn_fwd_f16(const void* q, const void* k, const void* v, void* o, float* lse,
                                     const int32_t* kv_lengths, const int64_t* dims, const int64_t* strides, float scale,
                                     int32_t dtype, void* stream);
+/* The gradients dq, dk, dv of asc_cuda_cross_attn_fwd_f16 from the gradient d_o of its output, its inputs, its output o
+ * and its lse (which must have been kept).  strides, in elements: d_o, q, k, v, o, dq, dk, dv (three each); alignment,
+ * dims, lengths and types as in the forward; d_o, q, dq, dk and dv must not repeat memory.  Where the batch or head
+ * stride of k or v is 0, dk and dv still hold a gradient per entry.  Keys from kv_lengths[b] on get a gradient of 0.  P and dS are rounded to dtype for their
+ * products, sums are fp32.  Every sum is taken in a fixed order (no atomics).  The workspace (8 bytes per query row, and
+ * fp32 parts where few rows are cut) is allocated and released on the stream.  Outputs must not overlap inputs. */
+int32_t asc_cuda_cross_attn_bwd_f16(const void* d_o, const void* q, const void* k, const void* v, const void* o,
+                                    const float* lse, const int32_t* kv_lengths, void* dq, void* dk, void* dv,
+                                    const int64_t* dims, const int64_t* strides, float scale, int32_t dtype,
+                                    void* stream);
 
 #ifdef __cplusplus
 }

@@ -110,3 +110,28 @@ def cross_attention_backward(do, q, k, v, lengths=None, scale=None):
     return (torch.einsum("bhst,bthd->bshd", ds, kc.repeat_interleave(group, 2)),
             grouped(torch.einsum("bhst,bshd->bthd", ds, q.double())),
             grouped(torch.einsum("bhst,bshd->bthd", p, do)))
+
+
+def cross_attention_backward_bounds(do, q, k, v, lengths, scale, step, least):
+    """How far dq, dk, dv may be off when P, dS, out and the results are rounded to a type with half a step of ``step``
+    (and ``least`` below its smallest normal), and scores, exponentials and sums are off by 2^-12 of their magnitudes:
+    dS is off by step |dS| + p (2^-12 (|dO| |V| + |dO| |P||V|) + 2 step |dO| |P||V|) + least, and dq, dk, dv by the sums
+    of that (of step p + 2^-12 p for dv) against |k|, |q|, |dO|, plus their own rounding."""
+    group = q.shape[2] // k.shape[2]
+    kc, vc = _clean(k, lengths), _clean(v, lengths)
+    ka, va, da = kc.abs().repeat_interleave(group, 2), vc.abs().repeat_interleave(group, 2), do.double().abs()
+    out, lse = cross_attention(q, k, v, lengths, scale)
+    p = torch.exp(_scores(q, kc, lengths, scale) - torch.where(lse == -math.inf, 0.0, lse)[..., None])
+    size = torch.einsum("bhst,bthd->bshd", p, va)
+    along = (da * size).sum(-1).transpose(1, 2)[..., None]
+    dp = torch.einsum("bshd,bthd->bhst", do.double(), vc.repeat_interleave(group, 2))
+    ds = p * (dp - (do.double() * out).sum(-1).transpose(1, 2)[..., None])
+    off = step * ds.abs() + p * (2.0**-12 * (torch.einsum("bshd,bthd->bhst", da, va) + along) + 2 * step * along) + least
+
+    def grouped(x):
+        return x.unflatten(2, (k.shape[2], group)).sum(3)
+
+    dq, dk, dv = cross_attention_backward(do, q, k, v, lengths, scale)
+    return (torch.einsum("bhst,bthd->bshd", off, ka) * scale + step * dq.abs() + least,
+            grouped(torch.einsum("bhst,bshd->bthd", off, q.double().abs())) * scale + step * dk.abs() + least,
+            grouped(torch.einsum("bhst,bshd->bthd", (step + 2.0**-12) * p + least, da)) + step * dv.abs() + least)

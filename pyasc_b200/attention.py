@@ -72,7 +72,7 @@ def _output(name: str, given: Optional[torch.Tensor], like: torch.Tensor, shape:
     return given
 
 
-_PACK = {n: struct.Struct(f"{n}q").pack for n in (6, 12, 14, 20)}     # host int64 arrays of the C ABI
+_PACK = {n: struct.Struct(f"{n}q").pack for n in (6, 12, 14, 20, 24)}     # host int64 arrays of the C ABI
 _NO_STRIDES = (0, 0, 0)
 
 
@@ -296,3 +296,28 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, kv_len
           _ptr(kv_lengths), dims, _PACK[12](*_strides(q), *_strides(k), *_strides(v), *_strides(out)), scale,
           _DTYPE_CODE[q.dtype])
     return (out, lse) if return_lse else out
+
+
+def cross_attention_backward(dout: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out: torch.Tensor,
+                             lse: torch.Tensor, *, kv_lengths: Optional[torch.Tensor] = None,
+                             scale: Optional[float] = None, dq: Optional[torch.Tensor] = None,
+                             dk: Optional[torch.Tensor] = None, dv: Optional[torch.Tensor] = None):
+    """Gradients ``(dq, dk, dv)`` of :func:`cross_attention`'s output from its gradient, its inputs, ``out`` and ``lse``
+    (of the same lengths and scale).  Keys that do not take part get 0; where k or v repeat one state over batch or heads,
+    dk and dv hold one gradient for each entry.  Every sum is taken in a fixed order.  The outputs must not overlap the
+    inputs."""
+    device, q_shape, k_shape, dims, scale = _cross_arguments(q, k, v, kv_lengths, scale)
+    dtype = q.dtype
+    _check_shape("dout", _check_rows("dout", dout, dtype, device), q_shape)
+    _check_shape("out", _check_rows("out", out, dtype, device), q_shape)
+    _check_vector("lse", lse, (torch.float32, ), device)
+    _check_shape("lse", lse.shape, (q_shape[0], q_shape[2], q_shape[1]))
+    if not lse.is_contiguous():
+        raise ValueError("lse must be contiguous")
+    dq = _output("dq", dq, q, q_shape, device)
+    dk, dv = _output("dk", dk, k, k_shape, device), _output("dv", dv, v, k_shape, device)
+    _call("asc_cuda_cross_attn_bwd_f16", device, dout.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(),
+          lse.data_ptr(), _ptr(kv_lengths), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), dims,
+          _PACK[24](*_strides(dout), *_strides(q), *_strides(k), *_strides(v), *_strides(out), *_strides(dq),
+                    *_strides(dk), *_strides(dv)), scale, _DTYPE_CODE[dtype])
+    return dq, dk, dv

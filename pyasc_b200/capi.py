@@ -74,6 +74,7 @@ PROTOTYPES: Dict[str, Sequence] = {
     "asc_cuda_attn_fwd_f16": (P, P, P, P, c_int32, c_int32, c_int32, c_int32, c_float, c_int32, c_int32, P),
     "asc_cuda_norm_rotary": (P, P, P, P, P, P, P, P, P, P, c_float, c_float, c_int32, c_int32, c_int32, P),
     "asc_cuda_cross_attn_fwd_f16": (P, P, P, P, P, P, P, P, c_float, c_int32, P),
+    "asc_cuda_cross_attn_bwd_f16": (P, P, P, P, P, P, P, P, P, P, P, P, c_float, c_int32, P),
     "asc_cuda_norm_rotary_bwd": (P, P, P, P, P, P, P, P, P, P, P, P, P, P, c_float, c_float, c_int32, c_int32, c_int32,
                                  P),
 }

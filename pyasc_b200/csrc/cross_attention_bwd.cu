@@ -1,0 +1,736 @@
+// Gradients of attention to another sequence (cross_attention.cu), fp16 / bf16, for sm_100a.  With P = exp(scale Q K^T -
+// lse) recomputed from the saved lse, and delta = rowsum(dO o O):
+//   dV = P^T dO,   dS = P o (dO V^T - delta),   dQ = scale dS K,   dK = scale dS^T Q.
+//
+// Two passes of one kernel, which differ in what stays and what streams:
+//   dQ      keeps 128 queries (Q, dO) and streams keys (K, V):   S = Q K^T, dP = dO V^T, dQ += dS K
+//   dK, dV  keeps 128 keys (K, V) and streams queries (Q, dO):   S = K Q^T, dP = V dO^T, dK += dS Q, dV += P dO
+// so that every sum stays in tensor memory and is written once: no atomics, the same bits in every run.  That costs seven
+// products instead of the five of a single pass; the five cannot keep all three sums on the SM, and adding dQ up across
+// SMs in memory would make its bits depend on the order.  dS and P are rounded to the inputs' type for their products.
+//
+// The stream comes in tiles of 64 rows, double buffered in tensor memory: two warpgroups take alternate steps, so the
+// exponentials of one step overlap the products of its neighbours.
+//   warps 0-3, 4-7   steps of even / odd number: scores and dP from tensor memory, dS and P back into the same columns;
+//                    at the end each writes one half of the sums
+//   warp 8           TMA producer: the kept tiles, then a ring of kStages stages (two tiles, and per query row its lse
+//                    and delta when queries stream)
+//   warp 9           MMA issuer
+// Few kept tiles are cut along the stream (`splits`): parts go to an fp32 workspace and are added up in order.
+// A small kernel first writes (lse in log2 units, delta) per query row, +inf for rows that must not count.
+#include "../../include/asc_cuda.h"
+#include "attention_common.cuh"
+#include "cross_attention.h"
+#include "host_common.h"
+
+namespace {
+
+using namespace ascdev;
+using namespace asccross;
+
+constexpr int kTile = 128;      // kept rows (= TMEM lanes)
+constexpr int kStep = 64;       // streamed rows per step
+constexpr int kThreads = 384;
+constexpr int kStages = 4;
+constexpr uint32_t kHalfStep = 64 * 128;    // 64 columns of a 64-row tile: 8 KiB
+constexpr uint32_t kColS = 0, kColAcc = 256;   // buffer b: S at 128 b, dP at 128 b + 64; sums at 256 and 384
+constexpr int kLaunchRegs = 168, kMathRegs = 208, kOtherRegs = 88;   // see attention.cu
+static_assert(8 * kMathRegs + 4 * kOtherRegs <= 12 * kLaunchRegs, "register split exceeds the launch allocation");
+
+struct BwdParams {
+  void* out[2];              // dQ, -  or  dK, dV
+  int64_t ob[2], os[2], oh[2];
+  float* part[2];            // splits > 1: [splits][B S H][D] unscaled sums (S, H of the kept side)
+  const float2* rows;        // [B, Hq, rows_pad] (lse log2 e or +inf, delta)
+  const int32_t* lengths;
+  int32_t B, Sq, Skv, Hkv, group, D;
+  int32_t rows_pad;
+  int32_t seg, pack;         // queries: rows per head and heads per tile (kept: of 128, streamed: of 64)
+  int32_t q_tiles;           // query tiles per (batch, key head)
+  int32_t q_tiles_per_head;  // pack == 1
+  int32_t kv_tiles;          // dK, dV: kept tiles of keys
+  int32_t splits, items;
+  int32_t k_heads, k_batches, v_heads, v_batches;
+  float scale, scale_log2;
+  uint32_t* status;
+};
+
+struct Item {
+  int b, hkv, tile;
+  int split, first, n;       // steps [first, first + n) of the stream
+  int len;
+};
+
+template <bool kKeys>
+__device__ __forceinline__ Item item_of(const BwdParams& p, int u) {
+  Item it;
+  const int tiles = kKeys ? p.kv_tiles : p.q_tiles;
+  const int per_head = tiles * p.splits;
+  const int bh = u / per_head, r = u - bh * per_head;
+  it.split = r / tiles;
+  it.tile = r - it.split * tiles;
+  it.b = bh / p.Hkv;
+  it.hkv = bh - it.b * p.Hkv;
+  int len = p.Skv;
+  if (p.lengths != nullptr) {
+    len = __ldg(p.lengths + it.b);
+    len = len < 0 ? 0 : len > p.Skv ? p.Skv : len;
+  }
+  it.len = len;
+  int total = kKeys ? p.q_tiles : (len + kStep - 1) / kStep;
+  if (kKeys && it.tile * kTile >= len) total = 0;          // all keys of the tile are gone
+  const int per = (total + p.splits - 1) / p.splits;
+  it.first = it.split * per;
+  const int left = total - it.first;
+  it.n = left < 0 ? 0 : left < per ? left : per;
+  return it;
+}
+
+// first head within its group and first query of a query tile of `rows` rows
+__device__ __forceinline__ void tile_origin(const BwdParams& p, int tile, int rows, int& head, int& s0) {
+  if (p.pack == 1) {
+    head = tile / p.q_tiles_per_head;
+    s0 = (tile - head * p.q_tiles_per_head) * rows;
+  } else {
+    head = tile * p.pack;
+    s0 = 0;
+  }
+}
+
+struct BwdCtl {
+  uint64_t r_full, r_empty;                       // kept tiles
+  uint64_t c_full[kStages], c_empty[kStages];     // stream
+  uint64_t s_full[2], p_full[2];                  // scores and dP written / dS and P written
+  uint64_t acc_full, acc_empty;
+  uint32_t tmem_base;
+  uint32_t abort_flag;
+};
+
+__device__ __forceinline__ void bulk_load(uint32_t dst_smem, const void* src, uint32_t bytes, uint32_t bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst_smem),
+               "l"(reinterpret_cast<uint64_t>(src)), "r"(bytes), "r"(bar)
+               : "memory");
+}
+__device__ __forceinline__ float4 ld_shared4(uint32_t addr) {
+  float4 v;
+  asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr));
+  return v;
+}
+
+// One step: 64 scores and dP of this thread's row -> dS (and P).
+template <bool kBf16, bool kKeys>
+__device__ __forceinline__ void step_math(uint32_t t_s, uint32_t pairs_smem, float2 row, float sl2, int limit) {
+#pragma unroll
+  for (int c = 0; c < 2; ++c) {
+    uint32_t s[32], d[32];
+    tmem_ld_32x32b_x32(t_s + c * 32, s);
+    tmem_ld_32x32b_x32(t_s + 64 + c * 32, d);
+    tmem_ld_wait();
+    uint32_t ds[16], pp[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      float2 l = make_float2(row.x, row.x), delta = make_float2(row.y, row.y);
+      if (kKeys) {
+        const float4 t = ld_shared4(pairs_smem + (c * 32 + 2 * i) * 8);
+        l = make_float2(t.x, t.z), delta = make_float2(t.y, t.w);
+      }
+      const float2 x = __ffma2_rn(make_float2(__uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1])),
+                                  make_float2(sl2, sl2), make_float2(-l.x, -l.y));
+      float2 e = make_float2(ex2_approx(x.x), ex2_approx(x.y));
+      float2 g = __fadd2_rn(make_float2(__uint_as_float(d[2 * i]), __uint_as_float(d[2 * i + 1])),
+                            make_float2(-delta.x, -delta.y));
+      if (!kKeys) {           // keys that are not there: whatever K and V hold, they count nothing
+        if (c * 32 + 2 * i > limit) e.x = g.x = 0.f;
+        if (c * 32 + 2 * i + 1 > limit) e.y = g.y = 0.f;
+      }
+      g = __fmul2_rn(e, g);
+      ds[i] = pack2<kBf16>(g.x, g.y);
+      if (kKeys) pp[i] = pack2<kBf16>(e.x, e.y);
+    }
+    tmem_st_32x32b_x16(t_s + c * 16, ds);
+    if (kKeys) tmem_st_32x32b_x16(t_s + 64 + c * 16, pp);
+  }
+}
+
+// Writes `kCols` columns of a sum for this thread's row, or zeros: for all rows (there was no step) or for a row that is
+// gone (its key is not there).
+template <bool kBf16, int kCols>
+__device__ __forceinline__ void write_row(const BwdParams& p, uint32_t t_acc, int which, int col0, bool valid, bool no_sum,
+                                          bool gone, int b, int s, int h, int64_t flat, float scale) {
+  const bool zero = no_sum || gone;
+  float* part = p.splits > 1 ? p.part[which] + flat * p.D : nullptr;
+  uint16_t* dst = static_cast<uint16_t*>(p.out[which]) + b * p.ob[which] + s * p.os[which] + h * p.oh[which];
+#pragma unroll 1
+  for (int c = 0; c < kCols; c += 32) {
+    uint32_t o[32];
+    if (!no_sum) {                 // warp-wide, also where the warp has rows that are gone
+      tmem_ld_32x32b_x32(t_acc + c, o);
+      tmem_ld_wait();
+    }
+    if (!valid) continue;
+    if (part != nullptr) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (col0 + c + i * 4 < p.D)
+          reinterpret_cast<uint4*>(part + col0 + c)[i] =
+              zero ? make_uint4(0, 0, 0, 0) : make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+    } else {
+      uint32_t pk[16];
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+        pk[i] = zero ? 0u : pack2<kBf16>(__uint_as_float(o[2 * i]) * scale, __uint_as_float(o[2 * i + 1]) * scale);
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (col0 + c + i * 8 < p.D)
+          reinterpret_cast<uint4*>(dst + col0 + c)[i] = make_uint4(pk[4 * i], pk[4 * i + 1], pk[4 * i + 2], pk[4 * i + 3]);
+    }
+  }
+}
+
+// tmap_r1 / r2: kept tiles, tmap_c1 / c2: stream.  kKeys: keys are kept (r = K, V; c = Q, dO), otherwise queries
+// (r = Q, dO; c = K, V).
+template <bool kBf16, int kHalves, bool kKeys>
+__global__ void __launch_bounds__(kThreads, 1)
+    cross_bwd_kernel(const __grid_constant__ CUtensorMap tmap_r1, const __grid_constant__ CUtensorMap tmap_r2,
+                     const __grid_constant__ CUtensorMap tmap_c1, const __grid_constant__ CUtensorMap tmap_c2,
+                     const BwdParams p, const uint32_t idesc_s, const uint32_t idesc_acc) {
+  constexpr uint32_t kKept = kHalves * kHalfTile, kStream = kHalves * kHalfStep;
+  constexpr uint32_t kSmemR = 0, kSmemC = 2 * kKept, kSmemPairs = kSmemC + kStages * 2 * kStream;
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ BwdCtl ctl;
+
+  const uint32_t warp = threadIdx.x >> 5;
+  const uint32_t lane = threadIdx.x & 31;
+  const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+  volatile uint32_t* abort_flag = &ctl.abort_flag;
+  const int stream_rows = kKeys ? p.seg * p.pack : kStep;      // rows of a stream tile: 16, 32, 48 or 64
+
+  if (threadIdx.x == 0) {
+    ctl.abort_flag = 0;
+    prefetch_tmap(&tmap_r1);
+    prefetch_tmap(&tmap_r2);
+    prefetch_tmap(&tmap_c1);
+    prefetch_tmap(&tmap_c2);
+    mbar_init(smem_u32(&ctl.r_full), 1);
+    mbar_init(smem_u32(&ctl.r_empty), 1);
+    mbar_init(smem_u32(&ctl.acc_full), 1);
+    mbar_init(smem_u32(&ctl.acc_empty), 256);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(smem_u32(&ctl.s_full[i]), 1);
+      mbar_init(smem_u32(&ctl.p_full[i]), 128);
+    }
+    for (int i = 0; i < kStages; ++i) {
+      mbar_init(smem_u32(&ctl.c_full[i]), 1);
+      mbar_init(smem_u32(&ctl.c_empty[i]), 1);
+    }
+    fence_mbar_init();
+  }
+  if (warp == 9) {
+    tmem_alloc(smem_u32(&ctl.tmem_base), 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_base = ctl.tmem_base;
+
+  // Every role walks the same list of items.  `g` numbers the steps of all items: it gives the buffer (g & 1), the
+  // warpgroup and the phases; `done` counts items with steps and gives the phases of the kept tiles and the sums.
+  if (warp < 8) {
+    setmaxnreg_inc<kMathRegs>();
+    const int wg = static_cast<int>(warp >> 2);
+    const int row = threadIdx.x & 127;
+    const uint32_t lane_base = ((threadIdx.x >> 5) & 3) * 32;
+    const uint32_t t_base = tmem_base + (lane_base << 16);
+    uint32_t g = 0, done = 0;
+    bool ok = true;
+    for (int u = blockIdx.x; u < p.items && ok; u += gridDim.x) {
+      const Item it = item_of<kKeys>(p, u);
+      int s, h;
+      bool valid;
+      float2 mine = make_float2(0.f, 0.f);
+      if (kKeys) {
+        s = it.tile * kTile + row;
+        h = it.hkv;
+        valid = s < p.Skv;
+      } else {
+        int head0, s0;
+        tile_origin(p, it.tile, kTile, head0, s0);
+        const int hl = head0 + row / p.seg;
+        s = s0 + row % p.seg;
+        valid = row < p.seg * p.pack && hl < p.group && s < p.Sq;
+        h = it.hkv * p.group + hl;
+        if (valid) mine = p.rows[(static_cast<int64_t>(it.b) * (p.Hkv * p.group) + h) * p.rows_pad + s];
+      }
+      for (int i = 0; i < it.n && ok; ++i) {
+        const uint32_t step = g + i, buf = step & 1;
+        if (static_cast<int>(buf) != wg) continue;
+        ok = mbar_wait(smem_u32(&ctl.s_full[buf]), (step >> 1) & 1, abort_flag, p.status, ASC_DEV_TIMEOUT_TMEM_FULL);
+        if (!ok) break;
+        if (kKeys) {           // the rows' lse and delta were written by the copy that this barrier counted
+          ok = mbar_wait(smem_u32(&ctl.c_full[step % kStages]), (step / kStages) & 1, abort_flag, p.status, ASC_DEV_TIMEOUT_FULL);
+          if (!ok) break;
+        }
+        tc_fence_after();
+        step_math<kBf16, kKeys>(t_base + kColS + buf * 128, smem_base + kSmemPairs + (step % kStages) * (kStep * 8), mine,
+                                p.scale_log2, kKeys ? 0 : it.len - 1 - (it.first + i) * kStep);
+        tmem_st_wait();
+        tc_fence_before();
+        mbar_arrive(smem_u32(&ctl.p_full[buf]));
+      }
+      if (!ok) break;
+      g += it.n;
+      const int64_t kept_heads = kKeys ? p.Hkv : p.Hkv * p.group, kept_seq = kKeys ? p.Skv : p.Sq;
+      const int64_t flat = ((static_cast<int64_t>(it.split) * p.B + it.b) * kept_seq + s) * kept_heads + h;
+      const bool zero = it.n == 0;
+      if (!zero) {
+        ok = mbar_wait(smem_u32(&ctl.acc_full), done & 1, abort_flag, p.status, ASC_DEV_TIMEOUT_TMEM_FULL);
+        if (!ok) break;
+        ++done;
+        tc_fence_after();
+      }
+      const bool gone = kKeys && s >= it.len;          // a key that is not there: its gradient is 0
+      if (kKeys) {
+        const uint32_t acc = t_base + kColAcc + wg * 128;
+        write_row<kBf16, 64 * kHalves>(p, acc, wg, 0, valid, zero, gone, it.b, s, h, flat, wg == 0 ? p.scale : 1.f);
+      } else {
+        const uint32_t acc = t_base + kColAcc + wg * 32 * kHalves;
+        write_row<kBf16, 32 * kHalves>(p, acc, 0, wg * 32 * kHalves, valid, zero, gone, it.b, s, h, flat, p.scale);
+      }
+      if (!zero) {
+        tc_fence_before();
+        mbar_arrive(smem_u32(&ctl.acc_empty));
+      }
+    }
+  } else {
+    setmaxnreg_dec<kOtherRegs>();
+    if (warp == 8) {
+      // ------------------------------ TMA producer ------------------------------
+      bool ok = true;
+      uint32_t done = 0;
+      Ring<kStages> ring;
+      const uint32_t kept_rows = kKeys ? kTile : static_cast<uint32_t>(p.seg * p.pack);
+      const uint32_t r_bytes = 2 * kept_rows * 128u * kHalves;
+      const uint32_t c_bytes = 2 * static_cast<uint32_t>(stream_rows) * 128u * kHalves + (kKeys ? stream_rows * 8u : 0u);
+      for (int u = blockIdx.x; u < p.items && ok; u += gridDim.x) {
+        const Item it = item_of<kKeys>(p, u);
+        if (it.n == 0) continue;
+        ok = mbar_wait(smem_u32(&ctl.r_empty), (done & 1) ^ 1, abort_flag, p.status, ASC_DEV_TIMEOUT_EMPTY);
+        if (!ok) break;
+        ++done;
+        if (lane == 0) {
+          const uint32_t bar = smem_u32(&ctl.r_full), dst = smem_base + kSmemR;
+          mbar_arrive_expect_tx(bar, r_bytes);
+          int head0 = 0, s0 = 0;
+          if (!kKeys) tile_origin(p, it.tile, kTile, head0, s0);
+#pragma unroll
+          for (int c = 0; c < kHalves; ++c) {
+            if (kKeys) {
+              tma_load_4d(dst + c * kHalfTile, &tmap_r1, bar, c * 64, it.tile * kTile, it.hkv * p.k_heads, it.b * p.k_batches);
+              tma_load_4d(dst + kKept + c * kHalfTile, &tmap_r2, bar, c * 64, it.tile * kTile, it.hkv * p.v_heads, it.b * p.v_batches);
+            } else {
+              tma_load_4d(dst + c * kHalfTile, &tmap_r1, bar, c * 64, s0, it.hkv * p.group + head0, it.b);
+              tma_load_4d(dst + kKept + c * kHalfTile, &tmap_r2, bar, c * 64, s0, it.hkv * p.group + head0, it.b);
+            }
+          }
+        }
+        __syncwarp();
+        for (int i = 0; i < it.n && ok; ++i) {
+          ok = mbar_wait(smem_u32(&ctl.c_empty[ring.stage]), ring.phase ^ 1, abort_flag, p.status, ASC_DEV_TIMEOUT_EMPTY);
+          if (!ok) break;
+          if (lane == 0) {
+            const uint32_t bar = smem_u32(&ctl.c_full[ring.stage]);
+            const uint32_t dst = smem_base + kSmemC + ring.stage * 2 * kStream;
+            mbar_arrive_expect_tx(bar, c_bytes);
+            int head0 = 0, s0 = (it.first + i) * kStep;
+            if (kKeys) tile_origin(p, it.first + i, kStep, head0, s0);
+            const int h0 = it.hkv * p.group + head0;
+#pragma unroll
+            for (int c = 0; c < kHalves; ++c) {
+              if (kKeys) {
+                tma_load_4d(dst + c * kHalfStep, &tmap_c1, bar, c * 64, s0, h0, it.b);
+                tma_load_4d(dst + kStream + c * kHalfStep, &tmap_c2, bar, c * 64, s0, h0, it.b);
+              } else {
+                tma_load_4d(dst + c * kHalfStep, &tmap_c1, bar, c * 64, s0, it.hkv * p.k_heads, it.b * p.k_batches);
+                tma_load_4d(dst + kStream + c * kHalfStep, &tmap_c2, bar, c * 64, s0, it.hkv * p.v_heads, it.b * p.v_batches);
+              }
+            }
+            if (kKeys)
+              bulk_load(smem_base + kSmemPairs + ring.stage * (kStep * 8),
+                        p.rows + (static_cast<int64_t>(it.b) * (p.Hkv * p.group) + h0) * p.rows_pad + s0, stream_rows * 8, bar);
+          }
+          ring.next();
+          __syncwarp();
+        }
+      }
+    } else if (warp == 9) {
+      // ------------------------------- MMA issuer -------------------------------
+      const uint64_t r_desc0 = make_smem_desc_sw128(smem_base + kSmemR, 16, 1024);
+      const uint64_t c_desc0 = make_smem_desc_sw128(smem_base + kSmemC, 16, 1024);             // as N x K, K-major
+      const uint64_t ct_desc0 = make_smem_desc_sw128(smem_base + kSmemC, kHalfStep, 1024);     // as K x N, MN-major
+      const int acc_steps = stream_rows / 16;
+      // S = R1 C1^T and dP = R2 C2^T into buffer `buf`
+      auto issue_scores = [&](uint32_t buf, uint32_t stage) {
+#pragma unroll
+        for (int m = 0; m < 2; ++m) {
+          const uint64_t rd = r_desc0 + ((m * kKept) >> 4);
+          const uint64_t cd = c_desc0 + ((stage * 2 * kStream + m * kStream) >> 4);
+          const uint32_t d = tmem_base + kColS + buf * 128 + m * 64;
+#pragma unroll
+          for (int ks = 0; ks < 4 * kHalves; ++ks)
+            umma_f16_ss(d, rd + (((ks >> 2) * kHalfTile + (ks & 3) * 32) >> 4),
+                        cd + (((ks >> 2) * kHalfStep + (ks & 3) * 32) >> 4), idesc_s, ks > 0 ? 1u : 0u);
+        }
+      };
+      // sums += dS C1 (and P C2)
+      auto issue_sums = [&](uint32_t buf, uint32_t stage, bool first) {
+#pragma unroll
+        for (int m = 0; m < (kKeys ? 2 : 1); ++m) {
+          const uint64_t cd = ct_desc0 + ((stage * 2 * kStream + m * kStream) >> 4);
+          const uint32_t a = tmem_base + kColS + buf * 128 + m * 64, d = tmem_base + kColAcc + m * 128;
+          for (int ks = 0; ks < acc_steps; ++ks)
+            umma_f16_ts(d, a + ks * 8, cd + ((ks * 2048) >> 4), idesc_acc, (!first || ks > 0) ? 1u : 0u);
+        }
+      };
+      bool ok = true;
+      uint32_t g = 0, done = 0;
+      Ring<kStages> s_ring, a_ring;        // stages in the order of their scores and of their sums
+      for (int u = blockIdx.x; u < p.items && ok; u += gridDim.x) {
+        const Item it = item_of<kKeys>(p, u);
+        if (it.n == 0) continue;
+        ok = mbar_wait(smem_u32(&ctl.r_full), done & 1, abort_flag, p.status, ASC_DEV_TIMEOUT_FULL);
+        if (!ok) break;
+        auto scores = [&](int i) {
+          ok = mbar_wait(smem_u32(&ctl.c_full[s_ring.stage]), s_ring.phase, abort_flag, p.status, ASC_DEV_TIMEOUT_FULL);
+          if (!ok) return;
+          if (!kKeys) {
+            const int here = it.len - (it.first + i) * kStep;
+            if (here < kStep && it.len < p.Skv) {
+              // rows of K past the length may hold anything, NaN too, and the zeros of dS would not silence that
+              const uint32_t base = smem_base + kSmemC + s_ring.stage * 2 * kStream;
+              for (int j = here * 8 + static_cast<int>(lane); j < kStep * 8; j += 32)
+#pragma unroll
+                for (int c = 0; c < kHalves; ++c) st_shared_zero16(base + c * kHalfStep + j * 16);
+              fence_proxy_async_smem();
+              __syncwarp();
+            }
+          }
+          tc_fence_after();
+          if (lane == 0) {
+            issue_scores((g + i) & 1, s_ring.stage);
+            umma_commit(smem_u32(&ctl.s_full[(g + i) & 1]));
+            if (i + 1 == it.n) umma_commit(smem_u32(&ctl.r_empty));      // the kept tiles' last use as an operand
+          }
+          __syncwarp();
+          s_ring.next();
+        };
+        for (int i = 0; i < 2 && i < it.n && ok; ++i) scores(i);
+        for (int i = 0; i < it.n && ok; ++i) {
+          const uint32_t step = g + i, buf = step & 1;
+          ok = mbar_wait(smem_u32(&ctl.p_full[buf]), (step >> 1) & 1, abort_flag, p.status, ASC_DEV_TIMEOUT_OTHER);
+          if (!ok) break;
+          if (i == 0) {            // the previous item's sums have been read
+            ok = mbar_wait(smem_u32(&ctl.acc_empty), (done & 1) ^ 1, abort_flag, p.status, ASC_DEV_TIMEOUT_TMEM_EMPTY);
+            if (!ok) break;
+          }
+          tc_fence_after();
+          if (lane == 0) {
+            issue_sums(buf, a_ring.stage, i == 0);
+            umma_commit(smem_u32(&ctl.c_empty[a_ring.stage]));
+            if (i + 1 == it.n) umma_commit(smem_u32(&ctl.acc_full));
+          }
+          __syncwarp();
+          a_ring.next();
+          if (i + 2 < it.n) scores(i + 2);
+        }
+        g += it.n;
+        ++done;
+      }
+    }
+  }
+
+  if (*abort_flag) {
+    const uint64_t t0 = global_timer_ns();
+    while (global_timer_ns() - t0 < 200000ull) __nanosleep(1000);
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 9) {
+    tc_fence_after();
+    tmem_dealloc(tmem_base, 512);
+  }
+}
+
+template <bool kBf16>
+__device__ __forceinline__ float dot2(uint32_t a, uint32_t b) {
+  if (kBf16)
+    return __uint_as_float(a << 16) * __uint_as_float(b << 16) + __uint_as_float(a & 0xffff0000u) * __uint_as_float(b & 0xffff0000u);
+  const float2 x = __half22float2(*reinterpret_cast<const __half2*>(&a)), y = __half22float2(*reinterpret_cast<const __half2*>(&b));
+  return x.x * y.x + x.y * y.y;
+}
+
+// (lse log2 e, delta) of every query row, a warp each; +inf and 0 for rows past the queries and rows without keys, whose
+// P is then 0.
+template <bool kBf16>
+__global__ void __launch_bounds__(256) cross_rows_kernel(const uint16_t* o, const uint16_t* dout, const float* lse,
+                                                         float2* rows, int64_t n, int Sq, int rows_pad, int Hq, int D,
+                                                         Strides os, Strides ds) {
+  const int lane = threadIdx.x & 31;
+  const int64_t i = blockIdx.x * 8ll + (threadIdx.x >> 5);
+  if (i >= n) return;
+  const int s = static_cast<int>(i % rows_pad);
+  const int64_t bh = i / rows_pad;
+  float2 r = make_float2(INFINITY, 0.f);
+  if (s < Sq) {
+    const int64_t b = bh / Hq, h = bh % Hq;
+    float t = 0.f;
+    if (lane * 4 < D) {
+      const uint2 x = *reinterpret_cast<const uint2*>(o + b * os.b + s * os.s + h * os.h + lane * 4);
+      const uint2 y = *reinterpret_cast<const uint2*>(dout + b * ds.b + s * ds.s + h * ds.h + lane * 4);
+      t = dot2<kBf16>(x.x, y.x) + dot2<kBf16>(x.y, y.y);
+    }
+#pragma unroll
+    for (int k = 16; k > 0; k >>= 1) t += __shfl_xor_sync(0xffffffffu, t, k);
+    const float l = lse[bh * Sq + s];
+    if (l != -INFINITY) r = make_float2(l * kLog2e, t);
+  }
+  if (lane == 0) rows[i] = r;
+}
+
+// out[row] = scale * sum of the parts in order; rows of [B, S, H], a warp each
+template <bool kBf16>
+__global__ void __launch_bounds__(256) cross_add_kernel(const float* part, uint16_t* out, int64_t n, int splits, int S, int H,
+                                                        int D, Strides st, float scale) {
+  const int c = (threadIdx.x & 31) * 4;
+  const int64_t i = blockIdx.x * 8ll + (threadIdx.x >> 5);
+  if (i >= n || c >= D) return;
+  float4 t = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int k = 0; k < splits; ++k) {
+    const float4 x = *reinterpret_cast<const float4*>(part + (k * n + i) * D + c);
+    t.x += x.x, t.y += x.y, t.z += x.z, t.w += x.w;
+  }
+  const int64_t h = i % H, bs = i / H;
+  *reinterpret_cast<uint2*>(out + bs / S * st.b + bs % S * st.s + h * st.h + c) =
+      make_uint2(pack2<kBf16>(t.x * scale, t.y * scale), pack2<kBf16>(t.z * scale, t.w * scale));
+}
+
+// ------------------------------------------------ host ---------------------------------------------------------
+// As in the forward, with a fixed cost of about six steps of 64 rows for an item (kept tiles, sums).
+int choose_splits(int64_t items, int64_t steps, int64_t sms) {
+  int best = 1;
+  int64_t best_cost = (items + sms - 1) / sms * (steps + 6);
+  for (int s = 2; s <= kMaxSplits && s <= steps; ++s) {
+    const int64_t cost = (items * s + sms - 1) / sms * ((steps + s - 1) / s + 6) + 8;
+    if (cost < best_cost) best_cost = cost, best = s;
+  }
+  return best;
+}
+
+template <bool kBf16, int kHalves, bool kKeys>
+int32_t launch_pass(const CUtensorMap& r1, const CUtensorMap& r2, const CUtensorMap& c1, const CUtensorMap& c2,
+                    const BwdParams& p, int sms, cudaStream_t stream) {
+  constexpr uint32_t smem = 2 * kHalves * kHalfTile + kStages * (2 * kHalves * kHalfStep + kStep * 8) + 1024;
+  auto kernel = cross_bwd_kernel<kBf16, kHalves, kKeys>;
+  static aschost::PerDevice attr_set;
+  int dev = 0;
+  ASC_CUDA_TRY(cudaGetDevice(&dev));
+  if (!attr_set.get(dev)) {
+    // refuse to launch a build whose register split would wait forever (see attention.cu)
+    cudaFuncAttributes fa{};
+    ASC_CUDA_TRY(cudaFuncGetAttributes(&fa, kernel));
+    if (12 * fa.numRegs < 8 * kMathRegs + 4 * kOtherRegs) return ASC_ERR_UNSUPPORTED;
+    ASC_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    attr_set.set(dev, 1);
+  }
+  const uint32_t fmt = kBf16 ? 1u : 0u;
+  const uint32_t idesc_s = make_idesc(1, fmt, fmt, 0, 0, kTile, kKeys ? p.seg * p.pack : kStep);
+  const uint32_t idesc_acc = make_idesc(1, fmt, fmt, 0, 1, kTile, 64 * kHalves);
+  const int grid = p.items < sms ? p.items : sms;
+  kernel<<<grid, kThreads, smem, stream>>>(r1, r2, c1, c2, p, idesc_s, idesc_acc);
+  aschost::count_launch();
+  ASC_CUDA_TRY(cudaGetLastError());
+  return ASC_OK;
+}
+
+template <bool kBf16, bool kKeys>
+int32_t launch_any(const CUtensorMap* maps, const BwdParams& p, int sms, cudaStream_t st) {
+  return p.D <= 64 ? launch_pass<kBf16, 1, kKeys>(maps[0], maps[1], maps[2], maps[3], p, sms, st)
+                   : launch_pass<kBf16, 2, kKeys>(maps[0], maps[1], maps[2], maps[3], p, sms, st);
+}
+
+struct Call {
+  const void *dout, *q, *k, *v, *o;
+  const float* lse;
+  void* grad[3];             // dq, dk, dv
+  int64_t B, Sq, Skv, Hq, Hkv, D;
+  Strides sdo, sq, sk, sv, so, sg[3];
+  const int32_t* lengths;
+  float scale;
+  cudaStream_t stream;
+};
+
+// Both passes on a workspace of `rows` (lse, delta) and, where a pass is cut, its parts.
+template <bool kBf16>
+int32_t run(const Call& c) {
+  int sms = 0;
+  int32_t rc = aschost::sm_count(&sms);
+  if (rc != ASC_OK) return rc;
+  const int64_t group = c.Hq / c.Hkv;
+  BwdParams p{};
+  p.lengths = c.lengths;
+  p.B = static_cast<int32_t>(c.B);
+  p.Sq = static_cast<int32_t>(c.Sq);
+  p.Skv = static_cast<int32_t>(c.Skv);
+  p.Hkv = static_cast<int32_t>(c.Hkv);
+  p.group = static_cast<int32_t>(group);
+  p.D = static_cast<int32_t>(c.D);
+  p.scale = c.scale;
+  p.scale_log2 = log2_scale(c.scale);
+  if ((rc = aschost::device_status_word(&p.status)) != ASC_OK) return rc;
+
+  // Queries in the stream: few queries share a tile of at most 64 rows over a number of heads that divides the group,
+  // each head's rows rounded up to 16 (the products' step), so that no row of a tile is undefined.
+  BwdParams pk = p, pq = p;
+  pk.seg = kStep, pk.pack = 1;
+  if (c.Sq <= kStep / 2) {
+    const int seg = static_cast<int>((c.Sq + 15) / 16 * 16);
+    int pack = kStep / seg;
+    while (group % pack != 0) --pack;
+    if (pack > 1) pk.seg = seg, pk.pack = pack;
+  }
+  const int64_t rows_pad = pk.pack > 1 ? pk.seg : (c.Sq + kStep - 1) / kStep * kStep;
+  pk.q_tiles_per_head = static_cast<int32_t>((c.Sq + kStep - 1) / kStep);
+  const int64_t k_steps = pk.pack > 1 ? group / pk.pack : group * pk.q_tiles_per_head;
+  const int64_t kv_tiles = (c.Skv + kTile - 1) / kTile;
+  // Queries kept: as in the forward
+  const int seg = static_cast<int>((c.Sq + 7) / 8 * 8 < kTile ? (c.Sq + 7) / 8 * 8 : kTile);
+  pq.pack = static_cast<int32_t>(kTile / seg < group ? kTile / seg : group);
+  pq.seg = pq.pack > 1 ? seg : kTile;
+  pq.q_tiles_per_head = static_cast<int32_t>((c.Sq + kTile - 1) / kTile);
+  const int64_t q_tiles = pq.pack > 1 ? (group + pq.pack - 1) / pq.pack : group * pq.q_tiles_per_head;
+  if (k_steps > (1 << 30) || c.B * c.Hkv * kv_tiles > 0x7fffffff / kMaxSplits ||
+      c.B * c.Hkv * q_tiles > 0x7fffffff / kMaxSplits || c.B * c.Hq > 0x7fffffff || c.B * c.Hq * rows_pad > (1ll << 33))
+    return ASC_ERR_TOO_LARGE;
+  pk.q_tiles = static_cast<int32_t>(k_steps);
+  pk.kv_tiles = static_cast<int32_t>(kv_tiles);
+  pq.q_tiles = static_cast<int32_t>(q_tiles);
+  pk.splits = choose_splits(c.B * c.Hkv * kv_tiles, k_steps, sms);
+  pq.splits = choose_splits(c.B * c.Hkv * q_tiles, (c.Skv + kStep - 1) / kStep, sms);
+  pk.items = static_cast<int32_t>(c.B * c.Hkv * kv_tiles * pk.splits);
+  pq.items = static_cast<int32_t>(c.B * c.Hkv * q_tiles * pq.splits);
+  pk.rows_pad = pq.rows_pad = static_cast<int32_t>(rows_pad);
+
+  // maps of each pass in its order: kept 1, kept 2, stream 1, stream 2
+  CUtensorMap mk[4], mq[4];
+  if (c.Skv > 0) {
+    if ((rc = encode_rows(&mk[0], kBf16, c.k, c.B, c.Skv, c.Hkv, c.D, c.sk, kTile, 1, &pk.k_heads, &pk.k_batches)) != ASC_OK ||
+        (rc = encode_rows(&mk[1], kBf16, c.v, c.B, c.Skv, c.Hkv, c.D, c.sv, kTile, 1, &pk.v_heads, &pk.v_batches)) != ASC_OK ||
+        (rc = encode_rows(&mk[2], kBf16, c.q, c.B, c.Sq, c.Hq, c.D, c.sq, pk.seg, pk.pack, nullptr, nullptr)) != ASC_OK ||
+        (rc = encode_rows(&mk[3], kBf16, c.dout, c.B, c.Sq, c.Hq, c.D, c.sdo, pk.seg, pk.pack, nullptr, nullptr)) != ASC_OK ||
+        (rc = encode_rows(&mq[2], kBf16, c.k, c.B, c.Skv, c.Hkv, c.D, c.sk, kStep, 1, &pq.k_heads, &pq.k_batches)) != ASC_OK ||
+        (rc = encode_rows(&mq[3], kBf16, c.v, c.B, c.Skv, c.Hkv, c.D, c.sv, kStep, 1, &pq.v_heads, &pq.v_batches)) != ASC_OK)
+      return rc;
+  }
+  if ((rc = encode_rows(&mq[0], kBf16, c.q, c.B, c.Sq, c.Hq, c.D, c.sq, pq.seg, pq.pack, nullptr, nullptr)) != ASC_OK ||
+      (rc = encode_rows(&mq[1], kBf16, c.dout, c.B, c.Sq, c.Hq, c.D, c.sdo, pq.seg, pq.pack, nullptr, nullptr)) != ASC_OK)
+    return rc;
+  if (c.Skv == 0) mq[2] = mq[3] = mq[0];        // never read: no item has a step
+
+  const size_t n_rows = static_cast<size_t>(c.B) * c.Hq * rows_pad;
+  const size_t n_q = static_cast<size_t>(c.B) * c.Sq * c.Hq, n_k = static_cast<size_t>(c.B) * c.Skv * c.Hkv;
+  const size_t rows_bytes = (n_rows * sizeof(float2) + 255) / 256 * 256;
+  const size_t q_bytes = pq.splits > 1 ? pq.splits * n_q * c.D * sizeof(float) : 0;
+  const size_t k_bytes = pk.splits > 1 ? pk.splits * n_k * c.D * sizeof(float) : 0;
+  void* ws = nullptr;
+  if ((rc = aschost::scratch_alloc(&ws, rows_bytes + q_bytes + 2 * k_bytes, c.stream)) != ASC_OK) return rc;
+  char* at = static_cast<char*>(ws);
+  pk.rows = pq.rows = reinterpret_cast<float2*>(at);
+  pq.part[0] = reinterpret_cast<float*>(at + rows_bytes);
+  pk.part[0] = reinterpret_cast<float*>(at + rows_bytes + q_bytes);
+  pk.part[1] = reinterpret_cast<float*>(at + rows_bytes + q_bytes + k_bytes);
+  for (int i = 0; i < 3; ++i) {
+    BwdParams& to = i == 0 ? pq : pk;
+    const int w = i == 2;
+    to.out[w] = c.grad[i];
+    to.ob[w] = c.sg[i].b, to.os[w] = c.sg[i].s, to.oh[w] = c.sg[i].h;
+  }
+  auto finish = [&](cudaError_t e, const char* what) {
+    if (e != cudaSuccess) return aschost::record_cuda_error(e, what);
+    aschost::count_launch();
+    return static_cast<int32_t>(ASC_OK);
+  };
+  auto add = [&](const float* part, int i, int64_t n, int splits, int64_t S, int64_t H, float scale) {
+    cross_add_kernel<kBf16><<<static_cast<unsigned>((n + 7) / 8), 256, 0, c.stream>>>(
+        part, static_cast<uint16_t*>(c.grad[i]), n, splits, static_cast<int>(S), static_cast<int>(H), static_cast<int>(c.D),
+        c.sg[i], scale);
+    return finish(cudaGetLastError(), "cross_add_kernel");
+  };
+  cross_rows_kernel<kBf16><<<static_cast<unsigned>((n_rows + 7) / 8), 256, 0, c.stream>>>(
+      static_cast<const uint16_t*>(c.o), static_cast<const uint16_t*>(c.dout), c.lse, const_cast<float2*>(pk.rows),
+      static_cast<int64_t>(n_rows), p.Sq, pk.rows_pad, static_cast<int>(c.Hq), p.D, c.so, c.sdo);
+  rc = finish(cudaGetLastError(), "cross_rows_kernel");
+  if (rc == ASC_OK && c.Skv > 0) rc = launch_any<kBf16, true>(mk, pk, sms, c.stream);
+  if (rc == ASC_OK) rc = launch_any<kBf16, false>(mq, pq, sms, c.stream);
+  if (rc == ASC_OK && pk.splits > 1) {
+    rc = add(pk.part[0], 1, n_k, pk.splits, c.Skv, c.Hkv, c.scale);
+    if (rc == ASC_OK) rc = add(pk.part[1], 2, n_k, pk.splits, c.Skv, c.Hkv, 1.f);
+  }
+  if (rc == ASC_OK && pq.splits > 1) rc = add(pq.part[0], 0, n_q, pq.splits, c.Sq, c.Hq, c.scale);
+  const int32_t freed = aschost::scratch_free(ws, c.stream);
+  return rc == ASC_OK ? freed : rc;
+}
+
+// Without a query the gradients of k and v are sums of nothing.
+template <bool kBf16>
+int32_t no_queries(const Call& c) {
+  const int64_t n = c.B * c.Skv * c.Hkv;
+  if ((n + 7) / 8 > 0x7fffffff) return ASC_ERR_TOO_LARGE;
+  for (int i = 1; i < 3; ++i) {
+    cross_add_kernel<kBf16><<<static_cast<unsigned>((n + 7) / 8), 256, 0, c.stream>>>(
+        nullptr, static_cast<uint16_t*>(c.grad[i]), n, 0, static_cast<int>(c.Skv), static_cast<int>(c.Hkv),
+        static_cast<int>(c.D), c.sg[i], 1.f);
+    ASC_CUDA_TRY(cudaGetLastError());
+    aschost::count_launch();
+  }
+  return ASC_OK;
+}
+
+}  // namespace
+
+extern "C" int32_t asc_cuda_cross_attn_bwd_f16(const void* d_o, const void* q, const void* k, const void* v, const void* o,
+                                               const float* lse, const int32_t* kv_lengths, void* dq, void* dk, void* dv,
+                                               const int64_t* dims, const int64_t* strides, float scale, int32_t dtype,
+                                               void* stream) {
+  int32_t rc = check_dims(dims, strides, scale, dtype);
+  if (rc != ASC_OK) return rc;
+  Call c{d_o, q, k, v, o, lse, {dq, dk, dv}, dims[0], dims[1], dims[2], dims[3], dims[4], dims[5], {}, {}, {}, {}, {}, {},
+         kv_lengths, scale, static_cast<cudaStream_t>(stream)};
+  if (c.B == 0 || c.Hkv == 0 || c.D == 0 || (c.Sq == 0 && c.Skv == 0) || (c.Hq == 0 && c.Skv == 0)) return ASC_OK;
+  // strides: dO, q, k, v, o, dq, dk, dv
+  c.sdo = strides_of(strides, c.B, c.Sq, c.Hq);
+  c.sq = strides_of(strides + 3, c.B, c.Sq, c.Hq);
+  c.sk = strides_of(strides + 6, c.B, c.Skv, c.Hkv);
+  c.sv = strides_of(strides + 9, c.B, c.Skv, c.Hkv);
+  c.so = strides_of(strides + 12, c.B, c.Sq, c.Hq);
+  c.sg[0] = strides_of(strides + 15, c.B, c.Sq, c.Hq);
+  c.sg[1] = strides_of(strides + 18, c.B, c.Skv, c.Hkv);
+  c.sg[2] = strides_of(strides + 21, c.B, c.Skv, c.Hkv);
+  const bool queries = c.Sq > 0 && c.Hq > 0;
+  if (c.Skv > 0) {
+    if ((rc = check_operand(dk, c.sg[1], c.B, c.Skv, c.Hkv, true)) != ASC_OK) return rc;
+    if ((rc = check_operand(dv, c.sg[2], c.B, c.Skv, c.Hkv, true)) != ASC_OK) return rc;
+    if (queries) {
+      if ((rc = check_operand(k, c.sk, c.B, c.Skv, c.Hkv, false)) != ASC_OK) return rc;
+      if ((rc = check_operand(v, c.sv, c.B, c.Skv, c.Hkv, false)) != ASC_OK) return rc;
+    }
+  }
+  if (!queries) return dtype == 1 ? no_queries<true>(c) : no_queries<false>(c);
+  // (queries and their gradients must not repeat memory; see the forward)
+  if ((rc = check_operand(q, c.sq, c.B, c.Sq, c.Hq, true)) != ASC_OK) return rc;
+  if ((rc = check_operand(d_o, c.sdo, c.B, c.Sq, c.Hq, true)) != ASC_OK) return rc;
+  if ((rc = check_operand(o, c.so, c.B, c.Sq, c.Hq, false)) != ASC_OK) return rc;
+  if ((rc = check_operand(dq, c.sg[0], c.B, c.Sq, c.Hq, true)) != ASC_OK) return rc;
+  if (lse == nullptr) return ASC_ERR_INVALID_ARG;
+  if (reinterpret_cast<uintptr_t>(lse) % 4 != 0 || reinterpret_cast<uintptr_t>(kv_lengths) % 4 != 0) return ASC_ERR_MISALIGNED;
+  return dtype == 1 ? run<true>(c) : run<false>(c);
+}
