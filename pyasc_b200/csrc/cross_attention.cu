@@ -206,7 +206,8 @@ __device__ __forceinline__ bool softmax_role(const CrossParams& p, Ctl& ctl, uin
     l += (l0 + l1) + (l2 + l3);
     tmem_st_wait();
     tc_fence_before();
-    mbar_arrive(smem_u32(&ctl.p_full[t]));
+    __syncwarp();
+    if ((threadIdx.x & 31) == 0) mbar_arrive(smem_u32(&ctl.p_full[t]));
   }
 
   if (it.n == 0) {
@@ -294,7 +295,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(smem_u32(&ctl.q_full[i]), 1);
       mbar_init(smem_u32(&ctl.q_empty[i]), 1);
       mbar_init(smem_u32(&ctl.s_full[i]), 1);
-      mbar_init(smem_u32(&ctl.p_full[i]), 128);
+      mbar_init(smem_u32(&ctl.p_full[i]), 4);
       mbar_init(smem_u32(&ctl.o_full[i]), 1);
     }
     for (int i = 0; i < kStages; ++i) {
@@ -344,7 +345,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           ok = mbar_wait(smem_u32(&ctl.q_empty[t]), (q_it[t] & 1) ^ 1, abort_flag, p.status, ASC_DEV_TIMEOUT_EMPTY);
           if (!ok) continue;
           ++q_it[t];
-          if (lane == 0) {
+          if (elect_one()) {
             int head0, s0;
             tile_origin(p, tile, head0, s0);
             const uint32_t bar = smem_u32(&ctl.q_full[t]);
@@ -360,7 +361,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           const int key = it.key0 + j * kTileKV;
           ok = mbar_wait(smem_u32(&ctl.k_empty[k_ring.stage]), k_ring.phase ^ 1, abort_flag, p.status, ASC_DEV_TIMEOUT_EMPTY);
           if (!ok) break;
-          if (lane == 0) {
+          if (elect_one()) {
             const uint32_t bar = smem_u32(&ctl.k_full[k_ring.stage]);
             const uint32_t dst = smem_base + kSmemK + k_ring.stage * kTileBytes;
             mbar_arrive_expect_tx(bar, kTileBytes);
@@ -371,7 +372,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           k_ring.next();
           ok = mbar_wait(smem_u32(&ctl.v_empty[v_ring.stage]), v_ring.phase ^ 1, abort_flag, p.status, ASC_DEV_TIMEOUT_EMPTY);
           if (!ok) break;
-          if (lane == 0) {
+          if (elect_one()) {
             const uint32_t bar = smem_u32(&ctl.v_full[v_ring.stage]);
             const uint32_t dst = smem_base + kSmemV + v_ring.stage * kTileBytes;
             mbar_arrive_expect_tx(bar, kTileBytes);
@@ -426,14 +427,14 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (!ok) continue;
           ++q_it[t];
           tc_fence_after();
-          if (lane == 0) {
+          if (elect_one()) {
             issue_qk(t, k_ring.stage);
             umma_commit(smem_u32(&ctl.s_full[t]));
             if (it.n == 1) umma_commit(smem_u32(&ctl.q_empty[t]));   // the tile's only Q K^T
           }
           __syncwarp();
         }
-        if (ok && lane == 0) umma_commit(smem_u32(&ctl.k_empty[k_ring.stage]));
+        if (ok && elect_one()) umma_commit(smem_u32(&ctl.k_empty[k_ring.stage]));
         __syncwarp();
         k_ring.next();
         for (int j = 0; j < it.n && ok; ++j) {
@@ -460,7 +461,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (!ok) continue;
             ++p_it[t];
             tc_fence_after();
-            if (lane == 0) {
+            if (elect_one()) {
               issue_pv(t, v_ring.stage, j > 0 ? 1u : 0u);
               if (j + 1 < it.n) {
                 issue_qk(t, k_ring.stage);
@@ -473,7 +474,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
             __syncwarp();
           }
-          if (ok && lane == 0) {
+          if (ok && elect_one()) {
             umma_commit(smem_u32(&ctl.v_empty[v_ring.stage]));
             if (j + 1 < it.n) umma_commit(smem_u32(&ctl.k_empty[k_ring.stage]));
           }

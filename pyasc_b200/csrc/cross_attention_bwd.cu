@@ -9,15 +9,16 @@
 // products instead of the five of a single pass; the five cannot keep all three sums on the SM, and adding dQ up across
 // SMs in memory would make its bits depend on the order.  dS and P are rounded to the inputs' type for their products.
 //
-// The stream comes in tiles of 64 rows, double buffered in tensor memory: two warpgroups take alternate steps, so the
-// exponentials of one step overlap the products of its neighbours.
-//   warps 0-3, 4-7   steps of even / odd number: scores and dP from tensor memory, dS and P back into the same columns;
-//                    at the end each writes one half of the sums
-//   warp 8           TMA producer: the kept tiles, then a ring of kStages stages (two tiles, and per query row its lse
-//                    and delta when queries stream)
-//   warp 9           MMA issuer
+// The stream comes in tiles of 64 rows, double buffered in tensor memory, so the exponentials of one step overlap the
+// products of its neighbours.  A step's 64 columns are halved between two warpgroups: what bounds a step is the chain
+// from its scores to its sums (its instructions fill a fifth of the issue slots), and half the columns are half the chain.
+//   warps 0-15   four warpgroups, (step parity) x (half of the columns): scores and dP from tensor memory, dS and P back
+//                into the same columns; at the end each writes a quarter of the sums
+//   warp 16      TMA producer: the kept tiles, then a ring of kStages stages (two tiles, and per query row its lse and
+//                delta when queries stream)
+//   warp 17      MMA issuer
 // Few kept tiles are cut along the stream (`splits`): parts go to an fp32 workspace and are added up in order.
-// A small kernel first writes (lse in log2 units, delta) per query row, +inf for rows that must not count.
+// A small kernel first writes -lse (in log2 units) and -delta per query row, -inf for rows that must not count.
 #include "../../include/asc_cuda.h"
 #include "attention_common.cuh"
 #include "cross_attention.h"
@@ -30,18 +31,20 @@ using namespace asccross;
 
 constexpr int kTile = 128;      // kept rows (= TMEM lanes)
 constexpr int kStep = 64;       // streamed rows per step
-constexpr int kThreads = 384;
+constexpr int kMathWarps = 16;
+constexpr int kThreads = (kMathWarps + 4) * 32;   // whole warpgroups: two warps idle
+// Register split after launch, see attention.cu: the increase may only take what the decrease releases.
+constexpr int kLaunchRegs = 96, kMathRegs = 104, kOtherRegs = 64;
+static_assert(kMathWarps * kMathRegs + 4 * kOtherRegs <= (kMathWarps + 4) * kLaunchRegs, "register split exceeds the launch allocation");
 constexpr int kStages = 4;
 constexpr uint32_t kHalfStep = 64 * 128;    // 64 columns of a 64-row tile: 8 KiB
 constexpr uint32_t kColS = 0, kColAcc = 256;   // buffer b: S at 128 b, dP at 128 b + 64; sums at 256 and 384
-constexpr int kLaunchRegs = 168, kMathRegs = 208, kOtherRegs = 88;   // see attention.cu
-static_assert(8 * kMathRegs + 4 * kOtherRegs <= 12 * kLaunchRegs, "register split exceeds the launch allocation");
-
 struct BwdParams {
   void* out[2];              // dQ, -  or  dK, dV
   int64_t ob[2], os[2], oh[2];
   float* part[2];            // splits > 1: [splits][B S H][D] unscaled sums (S, H of the kept side)
-  const float2* rows;        // [B, Hq, rows_pad] (lse log2 e or +inf, delta)
+  const float* rows_l;       // [B, Hq, rows_pad] -lse log2 e, or -inf
+  const float* rows_d;       // [B, Hq, rows_pad] -delta
   const int32_t* lengths;
   int32_t B, Sq, Skv, Hkv, group, D;
   int32_t rows_pad;
@@ -111,45 +114,43 @@ __device__ __forceinline__ void bulk_load(uint32_t dst_smem, const void* src, ui
                "l"(reinterpret_cast<uint64_t>(src)), "r"(bytes), "r"(bar)
                : "memory");
 }
-__device__ __forceinline__ float4 ld_shared4(uint32_t addr) {
-  float4 v;
-  asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr));
-  return v;
-}
-
-// One step: 64 scores and dP of this thread's row -> dS (and P).
+// Half a step: 32 scores and dP of this thread's row -> dS (and P), packed into the first 16 of the same columns.
+// (neg_l, neg_d): -lse and -delta of the row, or of the columns, from shared memory, when queries stream.
 template <bool kBf16, bool kKeys>
-__device__ __forceinline__ void step_math(uint32_t t_s, uint32_t pairs_smem, float2 row, float sl2, int limit) {
+__device__ __forceinline__ void step_math(uint32_t t_s, const float* col_l, const float* col_d, float neg_l, float neg_d,
+                                          float sl2, int limit) {
+  uint32_t s[32], d[32];
+  tmem_ld_32x32b_x32(t_s, s);
+  tmem_ld_32x32b_x32(t_s + 64, d);
+  tmem_ld_wait();
+  if (!kKeys && limit < 31) {       // keys that are not there: whatever K and V hold, they count nothing
 #pragma unroll
-  for (int c = 0; c < 2; ++c) {
-    uint32_t s[32], d[32];
-    tmem_ld_32x32b_x32(t_s + c * 32, s);
-    tmem_ld_32x32b_x32(t_s + 64 + c * 32, d);
-    tmem_ld_wait();
-    uint32_t ds[16], pp[16];
-#pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      float2 l = make_float2(row.x, row.x), delta = make_float2(row.y, row.y);
-      if (kKeys) {
-        const float4 t = ld_shared4(pairs_smem + (c * 32 + 2 * i) * 8);
-        l = make_float2(t.x, t.z), delta = make_float2(t.y, t.w);
-      }
-      const float2 x = __ffma2_rn(make_float2(__uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1])),
-                                  make_float2(sl2, sl2), make_float2(-l.x, -l.y));
-      float2 e = make_float2(ex2_approx(x.x), ex2_approx(x.y));
-      float2 g = __fadd2_rn(make_float2(__uint_as_float(d[2 * i]), __uint_as_float(d[2 * i + 1])),
-                            make_float2(-delta.x, -delta.y));
-      if (!kKeys) {           // keys that are not there: whatever K and V hold, they count nothing
-        if (c * 32 + 2 * i > limit) e.x = g.x = 0.f;
-        if (c * 32 + 2 * i + 1 > limit) e.y = g.y = 0.f;
-      }
-      g = __fmul2_rn(e, g);
-      ds[i] = pack2<kBf16>(g.x, g.y);
-      if (kKeys) pp[i] = pack2<kBf16>(e.x, e.y);
-    }
-    tmem_st_32x32b_x16(t_s + c * 16, ds);
-    if (kKeys) tmem_st_32x32b_x16(t_s + 64 + c * 16, pp);
+    for (int i = 0; i < 32; ++i)
+      if (i > limit) s[i] = 0xff800000u, d[i] = 0u;
   }
+  const float2 sl = make_float2(sl2, sl2);
+  uint32_t ds[16], pp[16];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    float4 l = make_float4(neg_l, neg_l, neg_l, neg_l), delta = make_float4(neg_d, neg_d, neg_d, neg_d);
+    if (kKeys) {
+      l = reinterpret_cast<const float4*>(col_l)[i];
+      delta = reinterpret_cast<const float4*>(col_d)[i];
+    }
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const int c = 4 * i + 2 * k;
+      const float2 lc = k == 0 ? make_float2(l.x, l.y) : make_float2(l.z, l.w);
+      const float2 dc = k == 0 ? make_float2(delta.x, delta.y) : make_float2(delta.z, delta.w);
+      const float2 x = __ffma2_rn(make_float2(__uint_as_float(s[c]), __uint_as_float(s[c + 1])), sl, lc);
+      const float2 e = make_float2(ex2_approx(x.x), ex2_approx(x.y));
+      const float2 g = __fmul2_rn(e, __fadd2_rn(make_float2(__uint_as_float(d[c]), __uint_as_float(d[c + 1])), dc));
+      ds[c / 2] = pack2<kBf16>(g.x, g.y);
+      if (kKeys) pp[c / 2] = pack2<kBf16>(e.x, e.y);
+    }
+  }
+  tmem_st_32x32b_x16(t_s, ds);
+  if (kKeys) tmem_st_32x32b_x16(t_s + 64, pp);
 }
 
 // Writes `kCols` columns of a sum for this thread's row, or zeros: for all rows (there was no step) or for a row that is
@@ -160,27 +161,27 @@ __device__ __forceinline__ void write_row(const BwdParams& p, uint32_t t_acc, in
   const bool zero = no_sum || gone;
   float* part = p.splits > 1 ? p.part[which] + flat * p.D : nullptr;
   uint16_t* dst = static_cast<uint16_t*>(p.out[which]) + b * p.ob[which] + s * p.os[which] + h * p.oh[which];
-#pragma unroll 1
-  for (int c = 0; c < kCols; c += 32) {
-    uint32_t o[32];
+#pragma unroll
+  for (int c = 0; c < kCols; c += 16) {
+    uint32_t o[16];
     if (!no_sum) {                 // warp-wide, also where the warp has rows that are gone
-      tmem_ld_32x32b_x32(t_acc + c, o);
+      tmem_ld_32x32b_x16(t_acc + c, o);
       tmem_ld_wait();
     }
     if (!valid) continue;
     if (part != nullptr) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i)
+      for (int i = 0; i < 4; ++i)
         if (col0 + c + i * 4 < p.D)
           reinterpret_cast<uint4*>(part + col0 + c)[i] =
               zero ? make_uint4(0, 0, 0, 0) : make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
     } else {
-      uint32_t pk[16];
+      uint32_t pk[8];
 #pragma unroll
-      for (int i = 0; i < 16; ++i)
+      for (int i = 0; i < 8; ++i)
         pk[i] = zero ? 0u : pack2<kBf16>(__uint_as_float(o[2 * i]) * scale, __uint_as_float(o[2 * i + 1]) * scale);
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
+      for (int i = 0; i < 2; ++i)
         if (col0 + c + i * 8 < p.D)
           reinterpret_cast<uint4*>(dst + col0 + c)[i] = make_uint4(pk[4 * i], pk[4 * i + 1], pk[4 * i + 2], pk[4 * i + 3]);
     }
@@ -214,10 +215,10 @@ __global__ void __launch_bounds__(kThreads, 1)
     mbar_init(smem_u32(&ctl.r_full), 1);
     mbar_init(smem_u32(&ctl.r_empty), 1);
     mbar_init(smem_u32(&ctl.acc_full), 1);
-    mbar_init(smem_u32(&ctl.acc_empty), 256);
+    mbar_init(smem_u32(&ctl.acc_empty), kMathWarps);
     for (int i = 0; i < 2; ++i) {
       mbar_init(smem_u32(&ctl.s_full[i]), 1);
-      mbar_init(smem_u32(&ctl.p_full[i]), 128);
+      mbar_init(smem_u32(&ctl.p_full[i]), kMathWarps / 2);
     }
     for (int i = 0; i < kStages; ++i) {
       mbar_init(smem_u32(&ctl.c_full[i]), 1);
@@ -225,7 +226,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     fence_mbar_init();
   }
-  if (warp == 9) {
+  if (warp == kMathWarps + 1) {
     tmem_alloc(smem_u32(&ctl.tmem_base), 512);
     tmem_relinquish();
   }
@@ -236,9 +237,10 @@ __global__ void __launch_bounds__(kThreads, 1)
 
   // Every role walks the same list of items.  `g` numbers the steps of all items: it gives the buffer (g & 1), the
   // warpgroup and the phases; `done` counts items with steps and gives the phases of the kept tiles and the sums.
-  if (warp < 8) {
+  if (warp < kMathWarps) {
     setmaxnreg_inc<kMathRegs>();
-    const int wg = static_cast<int>(warp >> 2);
+    const int parity = static_cast<int>(warp >> 2) & 1, half = static_cast<int>(warp >> 3);
+    const uint8_t* pairs = smem_raw + (smem_base - smem_u32(smem_raw)) + kSmemPairs + half * 32 * 4;
     const int row = threadIdx.x & 127;
     const uint32_t lane_base = ((threadIdx.x >> 5) & 3) * 32;
     const uint32_t t_base = tmem_base + (lane_base << 16);
@@ -246,25 +248,29 @@ __global__ void __launch_bounds__(kThreads, 1)
     bool ok = true;
     for (int u = blockIdx.x; u < p.items && ok; u += gridDim.x) {
       const Item it = item_of<kKeys>(p, u);
-      int s, h;
-      bool valid;
-      float2 mine = make_float2(0.f, 0.f);
-      if (kKeys) {
-        s = it.tile * kTile + row;
-        h = it.hkv;
-        valid = s < p.Skv;
-      } else {
+      // this thread's kept row: sequence position, head, and whether there is one
+      auto place = [&](int& s, int& h) {
+        if (kKeys) {
+          s = it.tile * kTile + row;
+          h = it.hkv;
+          return s < p.Skv;
+        }
         int head0, s0;
         tile_origin(p, it.tile, kTile, head0, s0);
         const int hl = head0 + row / p.seg;
         s = s0 + row % p.seg;
-        valid = row < p.seg * p.pack && hl < p.group && s < p.Sq;
         h = it.hkv * p.group + hl;
-        if (valid) mine = p.rows[(static_cast<int64_t>(it.b) * (p.Hkv * p.group) + h) * p.rows_pad + s];
+        return row < p.seg * p.pack && hl < p.group && s < p.Sq;
+      };
+      int s, h;
+      float neg_l = 0.f, neg_d = 0.f;
+      if (!kKeys && place(s, h)) {
+        const int64_t at = (static_cast<int64_t>(it.b) * (p.Hkv * p.group) + h) * p.rows_pad + s;
+        neg_l = p.rows_l[at], neg_d = p.rows_d[at];
       }
       for (int i = 0; i < it.n && ok; ++i) {
         const uint32_t step = g + i, buf = step & 1;
-        if (static_cast<int>(buf) != wg) continue;
+        if (static_cast<int>(buf) != parity) continue;
         ok = mbar_wait(smem_u32(&ctl.s_full[buf]), (step >> 1) & 1, abort_flag, p.status, ASC_DEV_TIMEOUT_TMEM_FULL);
         if (!ok) break;
         if (kKeys) {           // the rows' lse and delta were written by the copy that this barrier counted
@@ -272,14 +278,17 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (!ok) break;
         }
         tc_fence_after();
-        step_math<kBf16, kKeys>(t_base + kColS + buf * 128, smem_base + kSmemPairs + (step % kStages) * (kStep * 8), mine,
-                                p.scale_log2, kKeys ? 0 : it.len - 1 - (it.first + i) * kStep);
+        const float* cols = reinterpret_cast<const float*>(pairs + (step % kStages) * (kStep * 8));
+        step_math<kBf16, kKeys>(t_base + kColS + buf * 128 + half * 32, cols, cols + kStep, neg_l, neg_d, p.scale_log2,
+                                kKeys ? 0 : it.len - 1 - (it.first + i) * kStep - half * 32);
         tmem_st_wait();
         tc_fence_before();
-        mbar_arrive(smem_u32(&ctl.p_full[buf]));
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&ctl.p_full[buf]));
       }
       if (!ok) break;
       g += it.n;
+      const bool valid = place(s, h);
       const int64_t kept_heads = kKeys ? p.Hkv : p.Hkv * p.group, kept_seq = kKeys ? p.Skv : p.Sq;
       const int64_t flat = ((static_cast<int64_t>(it.split) * p.B + it.b) * kept_seq + s) * kept_heads + h;
       const bool zero = it.n == 0;
@@ -290,21 +299,23 @@ __global__ void __launch_bounds__(kThreads, 1)
         tc_fence_after();
       }
       const bool gone = kKeys && s >= it.len;          // a key that is not there: its gradient is 0
-      if (kKeys) {
-        const uint32_t acc = t_base + kColAcc + wg * 128;
-        write_row<kBf16, 64 * kHalves>(p, acc, wg, 0, valid, zero, gone, it.b, s, h, flat, wg == 0 ? p.scale : 1.f);
+      if (kKeys) {             // dK by the warpgroups of the first half, dV by the others; each one half of the columns
+        const int col0 = parity * 32 * kHalves;
+        write_row<kBf16, 32 * kHalves>(p, t_base + kColAcc + half * 128 + col0, half, col0, valid, zero, gone, it.b, s, h,
+                                       flat, half == 0 ? p.scale : 1.f);
       } else {
-        const uint32_t acc = t_base + kColAcc + wg * 32 * kHalves;
-        write_row<kBf16, 32 * kHalves>(p, acc, 0, wg * 32 * kHalves, valid, zero, gone, it.b, s, h, flat, p.scale);
+        const int col0 = (half * 2 + parity) * 16 * kHalves;
+        write_row<kBf16, 16 * kHalves>(p, t_base + kColAcc + col0, 0, col0, valid, zero, gone, it.b, s, h, flat, p.scale);
       }
       if (!zero) {
         tc_fence_before();
-        mbar_arrive(smem_u32(&ctl.acc_empty));
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&ctl.acc_empty));
       }
     }
   } else {
     setmaxnreg_dec<kOtherRegs>();
-    if (warp == 8) {
+    if (warp == kMathWarps) {
       // ------------------------------ TMA producer ------------------------------
       bool ok = true;
       uint32_t done = 0;
@@ -318,7 +329,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         ok = mbar_wait(smem_u32(&ctl.r_empty), (done & 1) ^ 1, abort_flag, p.status, ASC_DEV_TIMEOUT_EMPTY);
         if (!ok) break;
         ++done;
-        if (lane == 0) {
+        if (elect_one()) {
           const uint32_t bar = smem_u32(&ctl.r_full), dst = smem_base + kSmemR;
           mbar_arrive_expect_tx(bar, r_bytes);
           int head0 = 0, s0 = 0;
@@ -338,7 +349,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int i = 0; i < it.n && ok; ++i) {
           ok = mbar_wait(smem_u32(&ctl.c_empty[ring.stage]), ring.phase ^ 1, abort_flag, p.status, ASC_DEV_TIMEOUT_EMPTY);
           if (!ok) break;
-          if (lane == 0) {
+          if (elect_one()) {
             const uint32_t bar = smem_u32(&ctl.c_full[ring.stage]);
             const uint32_t dst = smem_base + kSmemC + ring.stage * 2 * kStream;
             mbar_arrive_expect_tx(bar, c_bytes);
@@ -355,15 +366,18 @@ __global__ void __launch_bounds__(kThreads, 1)
                 tma_load_4d(dst + kStream + c * kHalfStep, &tmap_c2, bar, c * 64, s0, it.hkv * p.v_heads, it.b * p.v_batches);
               }
             }
-            if (kKeys)
-              bulk_load(smem_base + kSmemPairs + ring.stage * (kStep * 8),
-                        p.rows + (static_cast<int64_t>(it.b) * (p.Hkv * p.group) + h0) * p.rows_pad + s0, stream_rows * 8, bar);
+            if (kKeys) {
+              const int64_t at = (static_cast<int64_t>(it.b) * (p.Hkv * p.group) + h0) * p.rows_pad + s0;
+              const uint32_t to = smem_base + kSmemPairs + ring.stage * (kStep * 8);
+              bulk_load(to, p.rows_l + at, stream_rows * 4, bar);
+              bulk_load(to + kStep * 4, p.rows_d + at, stream_rows * 4, bar);
+            }
           }
           ring.next();
           __syncwarp();
         }
       }
-    } else if (warp == 9) {
+    } else if (warp == kMathWarps + 1) {
       // ------------------------------- MMA issuer -------------------------------
       const uint64_t r_desc0 = make_smem_desc_sw128(smem_base + kSmemR, 16, 1024);
       const uint64_t c_desc0 = make_smem_desc_sw128(smem_base + kSmemC, 16, 1024);             // as N x K, K-major
@@ -388,8 +402,9 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int m = 0; m < (kKeys ? 2 : 1); ++m) {
           const uint64_t cd = ct_desc0 + ((stage * 2 * kStream + m * kStream) >> 4);
           const uint32_t a = tmem_base + kColS + buf * 128 + m * 64, d = tmem_base + kColAcc + m * 128;
-          for (int ks = 0; ks < acc_steps; ++ks)
-            umma_f16_ts(d, a + ks * 8, cd + ((ks * 2048) >> 4), idesc_acc, (!first || ks > 0) ? 1u : 0u);
+#pragma unroll
+          for (int ks = 0; ks < kStep / 16; ++ks)
+            if (ks < acc_steps) umma_f16_ts(d, a + (ks >> 1) * 32 + (ks & 1) * 8, cd + ((ks * 2048) >> 4), idesc_acc, (!first || ks > 0) ? 1u : 0u);
         }
       };
       bool ok = true;
@@ -416,7 +431,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
           }
           tc_fence_after();
-          if (lane == 0) {
+          if (elect_one()) {
             issue_scores((g + i) & 1, s_ring.stage);
             umma_commit(smem_u32(&ctl.s_full[(g + i) & 1]));
             if (i + 1 == it.n) umma_commit(smem_u32(&ctl.r_empty));      // the kept tiles' last use as an operand
@@ -434,7 +449,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (!ok) break;
           }
           tc_fence_after();
-          if (lane == 0) {
+          if (elect_one()) {
             issue_sums(buf, a_ring.stage, i == 0);
             umma_commit(smem_u32(&ctl.c_empty[a_ring.stage]));
             if (i + 1 == it.n) umma_commit(smem_u32(&ctl.acc_full));
@@ -455,7 +470,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
   tc_fence_before();
   __syncthreads();
-  if (warp == 9) {
+  if (warp == kMathWarps + 1) {
     tc_fence_after();
     tmem_dealloc(tmem_base, 512);
   }
@@ -469,18 +484,18 @@ __device__ __forceinline__ float dot2(uint32_t a, uint32_t b) {
   return x.x * y.x + x.y * y.y;
 }
 
-// (lse log2 e, delta) of every query row, a warp each; +inf and 0 for rows past the queries and rows without keys, whose
-// P is then 0.
+// -lse log2 e and -delta of every query row, a warp each; -inf and 0 for rows past the queries and rows without keys,
+// whose P is then 0.
 template <bool kBf16>
 __global__ void __launch_bounds__(256) cross_rows_kernel(const uint16_t* o, const uint16_t* dout, const float* lse,
-                                                         float2* rows, int64_t n, int Sq, int rows_pad, int Hq, int D,
+                                                         float* rows_l, float* rows_d, int64_t n, int Sq, int rows_pad, int Hq, int D,
                                                          Strides os, Strides ds) {
   const int lane = threadIdx.x & 31;
   const int64_t i = blockIdx.x * 8ll + (threadIdx.x >> 5);
   if (i >= n) return;
   const int s = static_cast<int>(i % rows_pad);
   const int64_t bh = i / rows_pad;
-  float2 r = make_float2(INFINITY, 0.f);
+  float2 r = make_float2(-INFINITY, 0.f);
   if (s < Sq) {
     const int64_t b = bh / Hq, h = bh % Hq;
     float t = 0.f;
@@ -492,9 +507,9 @@ __global__ void __launch_bounds__(256) cross_rows_kernel(const uint16_t* o, cons
 #pragma unroll
     for (int k = 16; k > 0; k >>= 1) t += __shfl_xor_sync(0xffffffffu, t, k);
     const float l = lse[bh * Sq + s];
-    if (l != -INFINITY) r = make_float2(l * kLog2e, t);
+    if (l != -INFINITY) r = make_float2(-l * kLog2e, -t);
   }
-  if (lane == 0) rows[i] = r;
+  if (elect_one()) rows_l[i] = r.x, rows_d[i] = r.y;
 }
 
 // out[row] = scale * sum of the parts in order; rows of [B, S, H], a warp each
@@ -538,7 +553,7 @@ int32_t launch_pass(const CUtensorMap& r1, const CUtensorMap& r2, const CUtensor
     // refuse to launch a build whose register split would wait forever (see attention.cu)
     cudaFuncAttributes fa{};
     ASC_CUDA_TRY(cudaFuncGetAttributes(&fa, kernel));
-    if (12 * fa.numRegs < 8 * kMathRegs + 4 * kOtherRegs) return ASC_ERR_UNSUPPORTED;
+    if ((kMathWarps + 4) * fa.numRegs < kMathWarps * kMathRegs + 4 * kOtherRegs) return ASC_ERR_UNSUPPORTED;
     ASC_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
     attr_set.set(dev, 1);
   }
@@ -638,13 +653,15 @@ int32_t run(const Call& c) {
 
   const size_t n_rows = static_cast<size_t>(c.B) * c.Hq * rows_pad;
   const size_t n_q = static_cast<size_t>(c.B) * c.Sq * c.Hq, n_k = static_cast<size_t>(c.B) * c.Skv * c.Hkv;
-  const size_t rows_bytes = (n_rows * sizeof(float2) + 255) / 256 * 256;
+  const size_t rows_bytes = (n_rows * 2 * sizeof(float) + 255) / 256 * 256;
   const size_t q_bytes = pq.splits > 1 ? pq.splits * n_q * c.D * sizeof(float) : 0;
   const size_t k_bytes = pk.splits > 1 ? pk.splits * n_k * c.D * sizeof(float) : 0;
   void* ws = nullptr;
   if ((rc = aschost::scratch_alloc(&ws, rows_bytes + q_bytes + 2 * k_bytes, c.stream)) != ASC_OK) return rc;
   char* at = static_cast<char*>(ws);
-  pk.rows = pq.rows = reinterpret_cast<float2*>(at);
+  float* rows = reinterpret_cast<float*>(at);
+  pk.rows_l = pq.rows_l = rows;
+  pk.rows_d = pq.rows_d = rows + n_rows;
   pq.part[0] = reinterpret_cast<float*>(at + rows_bytes);
   pk.part[0] = reinterpret_cast<float*>(at + rows_bytes + q_bytes);
   pk.part[1] = reinterpret_cast<float*>(at + rows_bytes + q_bytes + k_bytes);
@@ -666,7 +683,7 @@ int32_t run(const Call& c) {
     return finish(cudaGetLastError(), "cross_add_kernel");
   };
   cross_rows_kernel<kBf16><<<static_cast<unsigned>((n_rows + 7) / 8), 256, 0, c.stream>>>(
-      static_cast<const uint16_t*>(c.o), static_cast<const uint16_t*>(c.dout), c.lse, const_cast<float2*>(pk.rows),
+      static_cast<const uint16_t*>(c.o), static_cast<const uint16_t*>(c.dout), c.lse, rows, rows + n_rows,
       static_cast<int64_t>(n_rows), p.Sq, pk.rows_pad, static_cast<int>(c.Hq), p.D, c.so, c.sdo);
   rc = finish(cudaGetLastError(), "cross_rows_kernel");
   if (rc == ASC_OK && c.Skv > 0) rc = launch_any<kBf16, true>(mk, pk, sms, c.stream);

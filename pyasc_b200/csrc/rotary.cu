@@ -603,20 +603,30 @@ __global__ void __launch_bounds__(kThreads) rotary_any_kernel(const RotaryArgs a
 }
 
 // dgamma[w][c] = sum over the rows of partial sums of queries (w = 0; the first q_rows) or keys (w = 1), in a fixed
-// order: 8 interleaved sums in 64 bits
-__global__ void __launch_bounds__(256) dgamma_kernel(const float* partial, int q_rows, int rows, int D, float* dq_gamma,
-                                                     float* dk_gamma) {
-  __shared__ double red[8][32];
-  const int c = blockIdx.x * 32 + (threadIdx.x & 31), part = threadIdx.x >> 5;
+// order: 32 interleaved sums in 64 bits.  Latency-bound: a few hundred rows of D floats, so the loads of a thread are
+// independent of each other (eight at a time) and a CTA takes 32 columns.
+constexpr int kSumParts = 32;
+__global__ void __launch_bounds__(32 * kSumParts) dgamma_kernel(const float* partial, int q_rows, int rows, int D,
+                                                                float* dq_gamma, float* dk_gamma) {
+  __shared__ double red[kSumParts][32];
+  const int lane = threadIdx.x & 31, c = blockIdx.x * 32 + lane, part = threadIdx.x >> 5;
   const int lo = blockIdx.y ? q_rows : 0, hi = blockIdx.y ? rows : q_rows;
   float* out = blockIdx.y ? dk_gamma : dq_gamma;
   double t = 0.0;
   if (c < D)
-    for (int i = lo + part; i < hi; i += 8) t += partial[static_cast<int64_t>(i) * D + c];
-  red[part][threadIdx.x & 31] = t;
+    for (int i = lo + part; i < hi; i += 8 * kSumParts) {
+      float x[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k)
+        x[k] = i + k * kSumParts < hi ? partial[static_cast<int64_t>(i + k * kSumParts) * D + c] : 0.f;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) t += x[k];
+    }
+  red[part][lane] = t;
   __syncthreads();
   if (part == 0 && c < D && out != nullptr) {
-    for (int k = 1; k < 8; ++k) t += red[k][threadIdx.x & 31];
+#pragma unroll
+    for (int k = 1; k < kSumParts; ++k) t += red[k][lane];
     out[c] = static_cast<float>(t);
   }
 }
@@ -796,7 +806,7 @@ int32_t launch_bwd(RotaryArgs a, const Problem& pr, float* dq_gamma, float* dk_g
   if (e == cudaSuccess) {
     aschost::count_launch();
     if (ws != nullptr) {
-      dgamma_kernel<<<dim3((a.D + 31) / 32, 2), 256, 0, st>>>(a.partial, a.q_ctas, static_cast<int>(n_rows), a.D, dq_gamma,
+      dgamma_kernel<<<dim3((a.D + 31) / 32, 2), 32 * kSumParts, 0, st>>>(a.partial, a.q_ctas, static_cast<int>(n_rows), a.D, dq_gamma,
                                                               dk_gamma);
       e = cudaGetLastError();
       if (e == cudaSuccess) aschost::count_launch();
