@@ -271,12 +271,12 @@ __global__ void __launch_bounds__(kThreads, 1)
       for (int i = 0; i < it.n && ok; ++i) {
         const uint32_t step = g + i, buf = step & 1;
         if (static_cast<int>(buf) != parity) continue;
-        ok = mbar_wait(smem_u32(&ctl.s_full[buf]), (step >> 1) & 1, abort_flag, p.status, ASC_DEV_TIMEOUT_TMEM_FULL);
-        if (!ok) break;
-        if (kKeys) {           // the rows' lse and delta were written by the copy that this barrier counted
+        if (kKeys) {           // the rows' lse and delta were written by the copy that this barrier counts
           ok = mbar_wait(smem_u32(&ctl.c_full[step % kStages]), (step / kStages) & 1, abort_flag, p.status, ASC_DEV_TIMEOUT_FULL);
           if (!ok) break;
         }
+        ok = mbar_wait(smem_u32(&ctl.s_full[buf]), (step >> 1) & 1, abort_flag, p.status, ASC_DEV_TIMEOUT_TMEM_FULL);
+        if (!ok) break;
         tc_fence_after();
         const float* cols = reinterpret_cast<const float*>(pairs + (step % kStages) * (kStep * 8));
         step_math<kBf16, kKeys>(t_base + kColS + buf * 128 + half * 32, cols, cols + kStep, neg_l, neg_d, p.scale_log2,
@@ -315,8 +315,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
   } else {
     setmaxnreg_dec<kOtherRegs>();
-    if (warp == kMathWarps) {
-      // ------------------------------ TMA producer ------------------------------
+    if (warp == kMathWarps && elect_one()) {
+      // ------------------------------ TMA producer (one thread) ------------------------------
       bool ok = true;
       uint32_t done = 0;
       Ring<kStages> ring;
@@ -329,7 +329,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         ok = mbar_wait(smem_u32(&ctl.r_empty), (done & 1) ^ 1, abort_flag, p.status, ASC_DEV_TIMEOUT_EMPTY);
         if (!ok) break;
         ++done;
-        if (elect_one()) {
+        {
           const uint32_t bar = smem_u32(&ctl.r_full), dst = smem_base + kSmemR;
           mbar_arrive_expect_tx(bar, r_bytes);
           int head0 = 0, s0 = 0;
@@ -345,11 +345,10 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
           }
         }
-        __syncwarp();
         for (int i = 0; i < it.n && ok; ++i) {
           ok = mbar_wait(smem_u32(&ctl.c_empty[ring.stage]), ring.phase ^ 1, abort_flag, p.status, ASC_DEV_TIMEOUT_EMPTY);
           if (!ok) break;
-          if (elect_one()) {
+          {
             const uint32_t bar = smem_u32(&ctl.c_full[ring.stage]);
             const uint32_t dst = smem_base + kSmemC + ring.stage * 2 * kStream;
             mbar_arrive_expect_tx(bar, c_bytes);
@@ -374,15 +373,13 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
           }
           ring.next();
-          __syncwarp();
-        }
+          }
       }
-    } else if (warp == kMathWarps + 1) {
-      // ------------------------------- MMA issuer -------------------------------
+    } else if (warp == kMathWarps + 1 && elect_one()) {
+      // ------------------------------- MMA issuer (one thread) -------------------------------
       const uint64_t r_desc0 = make_smem_desc_sw128(smem_base + kSmemR, 16, 1024);
       const uint64_t c_desc0 = make_smem_desc_sw128(smem_base + kSmemC, 16, 1024);             // as N x K, K-major
       const uint64_t ct_desc0 = make_smem_desc_sw128(smem_base + kSmemC, kHalfStep, 1024);     // as K x N, MN-major
-      const int acc_steps = stream_rows / 16;
       // S = R1 C1^T and dP = R2 C2^T into buffer `buf`
       auto issue_scores = [&](uint32_t buf, uint32_t stage) {
 #pragma unroll
@@ -397,7 +394,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
       };
       // sums += dS C1 (and P C2)
-      auto issue_sums = [&](uint32_t buf, uint32_t stage, bool first) {
+      auto issue_sums = [&](uint32_t buf, uint32_t stage, int acc_steps, bool first) {
 #pragma unroll
         for (int m = 0; m < (kKeys ? 2 : 1); ++m) {
           const uint64_t cd = ct_desc0 + ((stage * 2 * kStream + m * kStream) >> 4);
@@ -415,48 +412,51 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (it.n == 0) continue;
         ok = mbar_wait(smem_u32(&ctl.r_full), done & 1, abort_flag, p.status, ASC_DEV_TIMEOUT_FULL);
         if (!ok) break;
-        auto scores = [&](int i) {
+        // Stage of step i has landed (and rows past the length are cleared).  Waited for before the wait on the math
+        // warps, so that nothing but that wait stands between their arrival and the next products.
+        auto landed = [&](int i) {
           ok = mbar_wait(smem_u32(&ctl.c_full[s_ring.stage]), s_ring.phase, abort_flag, p.status, ASC_DEV_TIMEOUT_FULL);
-          if (!ok) return;
-          if (!kKeys) {
-            const int here = it.len - (it.first + i) * kStep;
-            if (here < kStep && it.len < p.Skv) {
-              // rows of K past the length may hold anything, NaN too, and the zeros of dS would not silence that
-              const uint32_t base = smem_base + kSmemC + s_ring.stage * 2 * kStream;
-              for (int j = here * 8 + static_cast<int>(lane); j < kStep * 8; j += 32)
+          if (!ok || kKeys) return;
+          const int here = it.len - (it.first + i) * kStep;
+          if (here < kStep && it.len < p.Skv) {
+            // Rows of K past the length may hold anything, NaN too, and the zeros of dS would not silence that: the sums
+            // leave out whole groups of 16, the rest of the last group is cleared.
+            const uint32_t base = smem_base + kSmemC + s_ring.stage * 2 * kStream;
+            for (int j = here * 8; j < (here + 15) / 16 * 16 * 8; ++j)
 #pragma unroll
-                for (int c = 0; c < kHalves; ++c) st_shared_zero16(base + c * kHalfStep + j * 16);
-              fence_proxy_async_smem();
-              __syncwarp();
-            }
+              for (int c = 0; c < kHalves; ++c) st_shared_zero16(base + c * kHalfStep + j * 16);
+            fence_proxy_async_smem();
           }
-          tc_fence_after();
-          if (elect_one()) {
-            issue_scores((g + i) & 1, s_ring.stage);
-            umma_commit(smem_u32(&ctl.s_full[(g + i) & 1]));
-            if (i + 1 == it.n) umma_commit(smem_u32(&ctl.r_empty));      // the kept tiles' last use as an operand
-          }
-          __syncwarp();
-          s_ring.next();
         };
-        for (int i = 0; i < 2 && i < it.n && ok; ++i) scores(i);
+        auto scores = [&](int i) {
+          issue_scores((g + i) & 1, s_ring.stage);
+          umma_commit(smem_u32(&ctl.s_full[(g + i) & 1]));
+          if (i + 1 == it.n) umma_commit(smem_u32(&ctl.r_empty));      // the kept tiles' last use as an operand
+        };
+        for (int i = 0; i < 2 && i < it.n && ok; ++i) {
+          landed(i);
+          if (!ok) break;
+          tc_fence_after();
+          scores(i);
+          s_ring.next();
+        }
         for (int i = 0; i < it.n && ok; ++i) {
           const uint32_t step = g + i, buf = step & 1;
+          const bool more = i + 2 < it.n;
+          if (more) landed(i + 2);
+          if (ok && i == 0)        // the previous item's sums have been read
+            ok = mbar_wait(smem_u32(&ctl.acc_empty), (done & 1) ^ 1, abort_flag, p.status, ASC_DEV_TIMEOUT_TMEM_EMPTY);
+          if (!ok) break;
           ok = mbar_wait(smem_u32(&ctl.p_full[buf]), (step >> 1) & 1, abort_flag, p.status, ASC_DEV_TIMEOUT_OTHER);
           if (!ok) break;
-          if (i == 0) {            // the previous item's sums have been read
-            ok = mbar_wait(smem_u32(&ctl.acc_empty), (done & 1) ^ 1, abort_flag, p.status, ASC_DEV_TIMEOUT_TMEM_EMPTY);
-            if (!ok) break;
-          }
           tc_fence_after();
-          if (elect_one()) {
-            issue_sums(buf, a_ring.stage, i == 0);
-            umma_commit(smem_u32(&ctl.c_empty[a_ring.stage]));
-            if (i + 1 == it.n) umma_commit(smem_u32(&ctl.acc_full));
-          }
-          __syncwarp();
+          const int rows = kKeys ? stream_rows : min(kStep, it.len - (it.first + i) * kStep);
+          issue_sums(buf, a_ring.stage, (rows + 15) / 16, i == 0);
+          umma_commit(smem_u32(&ctl.c_empty[a_ring.stage]));
+          if (more) scores(i + 2);
+          else if (i + 1 == it.n) umma_commit(smem_u32(&ctl.acc_full));
           a_ring.next();
-          if (i + 2 < it.n) scores(i + 2);
+          if (more) s_ring.next();
         }
         g += it.n;
         ++done;
@@ -468,6 +468,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint64_t t0 = global_timer_ns();
     while (global_timer_ns() - t0 < 200000ull) __nanosleep(1000);
   }
+  __syncwarp();       // the lanes that issued come back to the others
   tc_fence_before();
   __syncthreads();
   if (warp == kMathWarps + 1) {
