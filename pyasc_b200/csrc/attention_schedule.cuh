@@ -100,11 +100,11 @@ struct Segment {
 struct Range {
   int pos, end, b, base;
 };
-__device__ __forceinline__ void find_range(const Schedule& s, Range* out) {
+__device__ __forceinline__ void find_range(const Schedule& s, int cta, int ctas, Range* out) {
   Range r{0, 0, 0, 0};
   if (s.whole < s.items) {
     const int total = total_steps(s);
-    const Position from = border(s, total, blockIdx.x, gridDim.x), to = border(s, total, blockIdx.x + 1, gridDim.x);
+    const Position from = border(s, total, cta, ctas), to = border(s, total, cta + 1, ctas);
     r = {from.pos, to.pos, from.b, from.base};
   }
   if ((threadIdx.x & 31) == 0) *out = r;
@@ -112,9 +112,10 @@ __device__ __forceinline__ void find_range(const Schedule& s, Range* out) {
 
 // The segments of a CTA, in the same order for every role.
 struct Walker {
-  int u, pos, end, start, b, base, tiles, steps, len;
+  int cta, ctas, u, pos, end, start, b, base, tiles, steps, len;
 
-  __device__ Walker(const Schedule& s, const Range& r) : u(blockIdx.x), pos(r.pos), end(r.end), start(r.pos), b(r.b), base(r.base) {
+  __device__ Walker(const Schedule& s, const Range& r, int cta_, int ctas_)
+      : cta(cta_), ctas(ctas_), u(cta_), pos(r.pos), end(r.end), start(r.pos), b(r.b), base(r.base) {
     if (pos < end) load(s);
   }
   __device__ void load(const Schedule& s) {
@@ -131,7 +132,7 @@ struct Walker {
       g.first = 0;
       g.n = g.tile < s.tiles_of(g.len) ? s.steps_of(g.len) : 0;
       g.slot = -1;
-      u += gridDim.x;
+      u += ctas;
       return true;
     }
     if (pos >= end) return false;
@@ -147,7 +148,7 @@ struct Walker {
     g.len = len;
     g.first = r - i * steps;
     g.n = min(steps - g.first, end - pos);
-    g.slot = g.n == steps ? -1 : 2 * static_cast<int>(blockIdx.x) + (pos != start);
+    g.slot = g.n == steps ? -1 : 2 * cta + (pos != start);
     pos += g.n;
     return true;
   }
@@ -156,9 +157,9 @@ struct Walker {
 // Items without steps among the divided ones (an entry without keys, a tile of keys past the length): their results are
 // zeros, which the CTAs write in turn.  `f(segment)` is called for each.
 template <typename F>
-__device__ __forceinline__ void for_empty_items(const Schedule& s, F&& f) {
+__device__ __forceinline__ void for_empty_items(const Schedule& s, int cta, int ctas, F&& f) {
   if (s.lengths == nullptr) return;
-  for (int u = s.whole + blockIdx.x; u < s.items; u += gridDim.x) {
+  for (int u = s.whole + cta; u < s.items; u += ctas) {
     Segment g;
     const int bh = u / s.tiles;
     g.tile = u - bh * s.tiles;
@@ -231,8 +232,9 @@ inline int plan(Schedule& s, int64_t steps_per_item, int sms, int64_t streamed_b
     }
   } else if (fits_l2 || items <= sms) {
     const int64_t work = items * steps_per_item;
-    s.whole = 0;
     s.cut = (work + sms - 1) / sms + 2 * item_cost + join_cost < cost_whole;
+    if (!s.cut && items <= sms) return s.items;       // one item each
+    s.whole = 0;
     const int64_t most = s.cut ? work : items;
     return static_cast<int>(most < sms ? most : sms);
   }

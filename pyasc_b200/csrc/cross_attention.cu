@@ -288,7 +288,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     tmem_alloc(smem_u32(&ctl.tmem_base), 512);
     tmem_relinquish();
   }
-  if (warp == 10) ascsched::find_range(p.work, &range);
+  if (warp == 10) ascsched::find_range(p.work, blockIdx.x, gridDim.x, &range);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -300,14 +300,14 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int t = static_cast<int>(warp >> 2);
     uint32_t s_it = 0, o_it = 0;
     bool ok = t < kTiles;
-    Walker walk(p.work, range);
+    Walker walk(p.work, range, blockIdx.x, gridDim.x);
     Segment it;
     while (ok && walk.next(p.work, it)) {
       const int tile = it.tile * kTiles + t;
       if (tile_exists(p, tile)) ok = softmax_role<kBf16, kHalves, kTiles>(p, ctl, tmem_base, t, it, tile, s_it, o_it);
     }
     if (ok)
-      ascsched::for_empty_items(p.work, [&](const Segment& e) {
+      ascsched::for_empty_items(p.work, blockIdx.x, gridDim.x, [&](const Segment& e) {
         const int tile = e.tile * kTiles + t;
         if (tile_exists(p, tile)) softmax_role<kBf16, kHalves, kTiles>(p, ctl, tmem_base, t, e, tile, s_it, o_it);
       });
@@ -319,7 +319,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       uint32_t q_it[2] = {0, 0};
       Ring<kStages> k_ring, v_ring;
       const uint32_t q_bytes = static_cast<uint32_t>(p.seg * p.pack) * 128u * kHalves;
-      Walker walk(p.work, range);
+      Walker walk(p.work, range, blockIdx.x, gridDim.x);
       Segment it;
       while (ok && walk.next(p.work, it)) {
         if (it.n == 0) continue;
@@ -398,7 +398,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       bool ok = true;
       uint32_t q_it[2] = {0, 0}, p_it[2] = {0, 0};
       Ring<kStages> k_ring, v_ring;
-      Walker walk(p.work, range);
+      Walker walk(p.work, range, blockIdx.x, gridDim.x);
       Segment it;
       while (ok && walk.next(p.work, it)) {
         if (it.n == 0) continue;
@@ -574,7 +574,7 @@ __global__ void __launch_bounds__(kFewWarps * 32, 2) cross_few_kernel(const Cros
   __shared__ Range range;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
   if (!kCluster) {
-    if (warp == 0) ascsched::find_range(p.work, &range);
+    if (warp == 0) ascsched::find_range(p.work, blockIdx.x, gridDim.x, &range);
     __syncthreads();
   }
   const int rows = p.group * p.Sq;
@@ -595,7 +595,7 @@ __global__ void __launch_bounds__(kFewWarps * 32, 2) cross_few_kernel(const Cros
     if ((threadIdx.x & 7) == 0 && p.lse != nullptr) p.lse[(static_cast<int64_t>(it.b) * (p.Hkv * p.group) + h) * p.Sq + s] = -INFINITY;
   };
 
-  Walker walk(p.work, kCluster ? Range{0, 0, 0, 0} : range);
+  Walker walk(p.work, kCluster ? Range{0, 0, 0, 0} : range, blockIdx.x, gridDim.x);
   Segment it;
   bool once = true;
   while (kCluster ? once : walk.next(p.work, it)) {
@@ -769,7 +769,7 @@ __global__ void __launch_bounds__(kFewWarps * 32, 2) cross_few_kernel(const Cros
     if (!kCluster) __syncthreads();               // the sums have been read
   }
   if (!kCluster) {
-    ascsched::for_empty_items(p.work, write_zero);
+    ascsched::for_empty_items(p.work, blockIdx.x, gridDim.x, write_zero);
     return;
   }
   // the parts of the cluster: rows in turn, D / 4 threads a row, CTAs in order

@@ -8,7 +8,6 @@ namespace asccross {
 
 constexpr uint32_t kHalfTile = 128 * 128;   // 64 columns of a 128-row 16-bit tile: 16 KiB
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr int kMaxSplits = 64;
 
 template <int kStages>
 struct Ring {

@@ -2,7 +2,8 @@
 // lse) recomputed from the saved lse, and delta = rowsum(dO o O):
 //   dV = P^T dO,   dS = P o (dO V^T - delta),   dQ = scale dS K,   dK = scale dS^T Q.
 //
-// Two passes of one kernel, which differ in what stays and what streams:
+// Two passes of one kernel (side by side in one launch, each on its share of the SMs), which differ in what stays and
+// what streams:
 //   dQ      keeps 128 queries (Q, dO) and streams keys (K, V):   S = Q K^T, dP = dO V^T, dQ += dS K
 //   dK, dV  keeps 128 keys (K, V) and streams queries (Q, dO):   S = K Q^T, dP = V dO^T, dK += dS Q, dV += P dO
 // so that every sum stays in tensor memory and is written once: no atomics, the same bits in every run.  That costs seven
@@ -17,10 +18,12 @@
 //   warp 16      TMA producer: the kept tiles, then a ring of kStages stages (two tiles, and per query row its lse and
 //                delta when queries stream)
 //   warp 17      MMA issuer
-// Few kept tiles are cut along the stream (`splits`): parts go to an fp32 workspace and are added up in order.
+// Where whole items (a kept tile and its stream) would leave SMs idle some are cut along the stream
+// (attention_schedule.cuh): parts go to an fp32 workspace and are added up in order.
 // A small kernel first writes -lse (in log2 units) and -delta per query row, -inf for rows that must not count.
 #include "../../include/asc_cuda.h"
 #include "attention_common.cuh"
+#include "attention_schedule.cuh"
 #include "cross_attention.h"
 #include "host_common.h"
 
@@ -28,6 +31,10 @@ namespace {
 
 using namespace ascdev;
 using namespace asccross;
+using ascsched::Range;
+using ascsched::Schedule;
+using ascsched::Segment;
+using ascsched::Walker;
 
 constexpr int kTile = 128;      // kept rows (= TMEM lanes)
 constexpr int kStep = 64;       // streamed rows per step
@@ -42,52 +49,18 @@ constexpr uint32_t kColS = 0, kColAcc = 256;   // buffer b: S at 128 b, dP at 12
 struct BwdParams {
   void* out[2];              // dQ, -  or  dK, dV
   int64_t ob[2], os[2], oh[2];
-  float* part[2];            // splits > 1: [splits][B S H][D] unscaled sums (S, H of the kept side)
+  float* part;               // parts: [slot][sum][128 rows][D], unscaled
+  Schedule work;
   const float* rows_l;       // [B, Hq, rows_pad] -lse log2 e, or -inf
   const float* rows_d;       // [B, Hq, rows_pad] -delta
-  const int32_t* lengths;
   int32_t B, Sq, Skv, Hkv, group, D;
   int32_t rows_pad;
   int32_t seg, pack;         // queries: rows per head and heads per tile (kept: of 128, streamed: of 64)
-  int32_t q_tiles;           // query tiles per (batch, key head)
   int32_t q_tiles_per_head;  // pack == 1
-  int32_t kv_tiles;          // dK, dV: kept tiles of keys
-  int32_t splits, items;
   int32_t k_heads, k_batches, v_heads, v_batches;
   float scale, scale_log2;
   uint32_t* status;
 };
-
-struct Item {
-  int b, hkv, tile;
-  int split, first, n;       // steps [first, first + n) of the stream
-  int len;
-};
-
-template <bool kKeys>
-__device__ __forceinline__ Item item_of(const BwdParams& p, int u) {
-  Item it;
-  const int tiles = kKeys ? p.kv_tiles : p.q_tiles;
-  const int per_head = tiles * p.splits;
-  const int bh = u / per_head, r = u - bh * per_head;
-  it.split = r / tiles;
-  it.tile = r - it.split * tiles;
-  it.b = bh / p.Hkv;
-  it.hkv = bh - it.b * p.Hkv;
-  int len = p.Skv;
-  if (p.lengths != nullptr) {
-    len = __ldg(p.lengths + it.b);
-    len = len < 0 ? 0 : len > p.Skv ? p.Skv : len;
-  }
-  it.len = len;
-  int total = kKeys ? p.q_tiles : (len + kStep - 1) / kStep;
-  if (kKeys && it.tile * kTile >= len) total = 0;          // all keys of the tile are gone
-  const int per = (total + p.splits - 1) / p.splits;
-  it.first = it.split * per;
-  const int left = total - it.first;
-  it.n = left < 0 ? 0 : left < per ? left : per;
-  return it;
-}
 
 // first head within its group and first query of a query tile of `rows` rows
 __device__ __forceinline__ void tile_origin(const BwdParams& p, int tile, int rows, int& head, int& s0) {
@@ -98,6 +71,22 @@ __device__ __forceinline__ void tile_origin(const BwdParams& p, int tile, int ro
     head = tile * p.pack;
     s0 = 0;
   }
+}
+
+// Sequence position and head of a kept tile's row; false where there is none.
+template <bool kKeys>
+__device__ __forceinline__ bool row_place(const BwdParams& p, const Segment& it, int row, int& s, int& h) {
+  if (kKeys) {
+    s = it.tile * kTile + row;
+    h = it.hkv;
+    return s < p.Skv;
+  }
+  int head0, s0;
+  tile_origin(p, it.tile, kTile, head0, s0);
+  const int hl = head0 + row / p.seg;
+  s = s0 + row % p.seg;
+  h = it.hkv * p.group + hl;
+  return row < p.seg * p.pack && hl < p.group && s < p.Sq;
 }
 
 struct BwdCtl {
@@ -157,9 +146,8 @@ __device__ __forceinline__ void step_math(uint32_t t_s, const float* col_l, cons
 // gone (its key is not there).
 template <bool kBf16, int kCols>
 __device__ __forceinline__ void write_row(const BwdParams& p, uint32_t t_acc, int which, int col0, bool valid, bool no_sum,
-                                          bool gone, int b, int s, int h, int64_t flat, float scale) {
+                                          bool gone, int b, int s, int h, float* part, float scale) {
   const bool zero = no_sum || gone;
-  float* part = p.splits > 1 ? p.part[which] + flat * p.D : nullptr;
   uint16_t* dst = static_cast<uint16_t*>(p.out[which]) + b * p.ob[which] + s * p.os[which] + h * p.oh[which];
 #pragma unroll
   for (int c = 0; c < kCols; c += 16) {
@@ -188,18 +176,20 @@ __device__ __forceinline__ void write_row(const BwdParams& p, uint32_t t_acc, in
   }
 }
 
-// tmap_r1 / r2: kept tiles, tmap_c1 / c2: stream.  kKeys: keys are kept (r = K, V; c = Q, dO), otherwise queries
-// (r = Q, dO; c = K, V).
+// Tensor maps of a pass: kept tiles 1 and 2, stream 1 and 2.  Keys kept: K, V; Q, dO.  Queries kept: Q, dO; K, V.
+struct Maps {
+  CUtensorMap r1, r2, c1, c2;
+};
+
 template <bool kBf16, int kHalves, bool kKeys>
-__global__ void __launch_bounds__(kThreads, 1)
-    cross_bwd_kernel(const __grid_constant__ CUtensorMap tmap_r1, const __grid_constant__ CUtensorMap tmap_r2,
-                     const __grid_constant__ CUtensorMap tmap_c1, const __grid_constant__ CUtensorMap tmap_c2,
-                     const BwdParams p, const uint32_t idesc_s, const uint32_t idesc_acc) {
+__device__ __forceinline__ void bwd_pass(const Maps& maps, const BwdParams& p, const int cta, const int ctas,
+                                         uint8_t* smem_raw, BwdCtl& ctl, Range& range) {
+  const CUtensorMap &tmap_r1 = maps.r1, &tmap_r2 = maps.r2, &tmap_c1 = maps.c1, &tmap_c2 = maps.c2;
+  constexpr uint32_t kFmt = kBf16 ? 1u : 0u;
+  const uint32_t idesc_s = make_idesc(1, kFmt, kFmt, 0, 0, kTile, kKeys ? p.seg * p.pack : kStep);
+  constexpr uint32_t idesc_acc = make_idesc(1, kFmt, kFmt, 0, 1, kTile, 64 * kHalves);
   constexpr uint32_t kKept = kHalves * kHalfTile, kStream = kHalves * kHalfStep;
   constexpr uint32_t kSmemR = 0, kSmemC = 2 * kKept, kSmemPairs = kSmemC + kStages * 2 * kStream;
-  extern __shared__ uint8_t smem_raw[];
-  __shared__ BwdCtl ctl;
-
   const uint32_t warp = threadIdx.x >> 5;
   const uint32_t lane = threadIdx.x & 31;
   const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
@@ -230,13 +220,14 @@ __global__ void __launch_bounds__(kThreads, 1)
     tmem_alloc(smem_u32(&ctl.tmem_base), 512);
     tmem_relinquish();
   }
+  if (warp == kMathWarps) ascsched::find_range(p.work, cta, ctas, &range);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem_base = ctl.tmem_base;
 
-  // Every role walks the same list of items.  `g` numbers the steps of all items: it gives the buffer (g & 1), the
-  // warpgroup and the phases; `done` counts items with steps and gives the phases of the kept tiles and the sums.
+  // Every role walks the same list of segments.  `g` numbers the steps of all segments: it gives the buffer (g & 1), the
+  // warpgroup and the phases; `done` counts segments with steps and gives the phases of the kept tiles and the sums.
   if (warp < kMathWarps) {
     setmaxnreg_inc<kMathRegs>();
     const int parity = static_cast<int>(warp >> 2) & 1, half = static_cast<int>(warp >> 3);
@@ -246,25 +237,29 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t t_base = tmem_base + (lane_base << 16);
     uint32_t g = 0, done = 0;
     bool ok = true;
-    for (int u = blockIdx.x; u < p.items && ok; u += gridDim.x) {
-      const Item it = item_of<kKeys>(p, u);
-      // this thread's kept row: sequence position, head, and whether there is one
-      auto place = [&](int& s, int& h) {
-        if (kKeys) {
-          s = it.tile * kTile + row;
-          h = it.hkv;
-          return s < p.Skv;
-        }
-        int head0, s0;
-        tile_origin(p, it.tile, kTile, head0, s0);
-        const int hl = head0 + row / p.seg;
-        s = s0 + row % p.seg;
-        h = it.hkv * p.group + hl;
-        return row < p.seg * p.pack && hl < p.group && s < p.Sq;
-      };
+    // writes a segment's sums, or zeros where there is no step
+    auto finish = [&](const Segment& it) {
+      int s, h;
+      const bool valid = row_place<kKeys>(p, it, row, s, h);
+      const bool gone = kKeys && s >= it.len;          // a key that is not there: its gradient is 0
+      float* part = nullptr;
+      if (it.slot >= 0) part = p.part + (static_cast<int64_t>(it.slot) * (kKeys ? 2 : 1) * kTile + row) * p.D;
+      if (kKeys) {             // dK by the warpgroups of the first half, dV by the others; each one half of the columns
+        const int col0 = parity * 32 * kHalves;
+        if (part != nullptr) part += half * kTile * p.D;
+        write_row<kBf16, 32 * kHalves>(p, t_base + kColAcc + half * 128 + col0, half, col0, valid, it.n == 0, gone, it.b, s, h,
+                                       part, half == 0 ? p.scale : 1.f);
+      } else {
+        const int col0 = (half * 2 + parity) * 16 * kHalves;
+        write_row<kBf16, 16 * kHalves>(p, t_base + kColAcc + col0, 0, col0, valid, it.n == 0, gone, it.b, s, h, part, p.scale);
+      }
+    };
+    Walker walk(p.work, range, cta, ctas);
+    Segment it;
+    while (ok && walk.next(p.work, it)) {
       int s, h;
       float neg_l = 0.f, neg_d = 0.f;
-      if (!kKeys && place(s, h)) {
+      if (!kKeys && row_place<kKeys>(p, it, row, s, h)) {
         const int64_t at = (static_cast<int64_t>(it.b) * (p.Hkv * p.group) + h) * p.rows_pad + s;
         neg_l = p.rows_l[at], neg_d = p.rows_d[at];
       }
@@ -288,9 +283,6 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       if (!ok) break;
       g += it.n;
-      const bool valid = place(s, h);
-      const int64_t kept_heads = kKeys ? p.Hkv : p.Hkv * p.group, kept_seq = kKeys ? p.Skv : p.Sq;
-      const int64_t flat = ((static_cast<int64_t>(it.split) * p.B + it.b) * kept_seq + s) * kept_heads + h;
       const bool zero = it.n == 0;
       if (!zero) {
         ok = mbar_wait(smem_u32(&ctl.acc_full), done & 1, abort_flag, p.status, ASC_DEV_TIMEOUT_TMEM_FULL);
@@ -298,21 +290,14 @@ __global__ void __launch_bounds__(kThreads, 1)
         ++done;
         tc_fence_after();
       }
-      const bool gone = kKeys && s >= it.len;          // a key that is not there: its gradient is 0
-      if (kKeys) {             // dK by the warpgroups of the first half, dV by the others; each one half of the columns
-        const int col0 = parity * 32 * kHalves;
-        write_row<kBf16, 32 * kHalves>(p, t_base + kColAcc + half * 128 + col0, half, col0, valid, zero, gone, it.b, s, h,
-                                       flat, half == 0 ? p.scale : 1.f);
-      } else {
-        const int col0 = (half * 2 + parity) * 16 * kHalves;
-        write_row<kBf16, 16 * kHalves>(p, t_base + kColAcc + col0, 0, col0, valid, zero, gone, it.b, s, h, flat, p.scale);
-      }
+      finish(it);
       if (!zero) {
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(smem_u32(&ctl.acc_empty));
       }
     }
+    if (ok) ascsched::for_empty_items(p.work, cta, ctas, finish);
   } else {
     setmaxnreg_dec<kOtherRegs>();
     if (warp == kMathWarps && elect_one()) {
@@ -323,8 +308,9 @@ __global__ void __launch_bounds__(kThreads, 1)
       const uint32_t kept_rows = kKeys ? kTile : static_cast<uint32_t>(p.seg * p.pack);
       const uint32_t r_bytes = 2 * kept_rows * 128u * kHalves;
       const uint32_t c_bytes = 2 * static_cast<uint32_t>(stream_rows) * 128u * kHalves + (kKeys ? stream_rows * 8u : 0u);
-      for (int u = blockIdx.x; u < p.items && ok; u += gridDim.x) {
-        const Item it = item_of<kKeys>(p, u);
+      Walker walk(p.work, range, cta, ctas);
+      Segment it;
+      while (ok && walk.next(p.work, it)) {
         if (it.n == 0) continue;
         ok = mbar_wait(smem_u32(&ctl.r_empty), (done & 1) ^ 1, abort_flag, p.status, ASC_DEV_TIMEOUT_EMPTY);
         if (!ok) break;
@@ -407,8 +393,9 @@ __global__ void __launch_bounds__(kThreads, 1)
       bool ok = true;
       uint32_t g = 0, done = 0;
       Ring<kStages> s_ring, a_ring;        // stages in the order of their scores and of their sums
-      for (int u = blockIdx.x; u < p.items && ok; u += gridDim.x) {
-        const Item it = item_of<kKeys>(p, u);
+      Walker walk(p.work, range, cta, ctas);
+      Segment it;
+      while (ok && walk.next(p.work, it)) {
         if (it.n == 0) continue;
         ok = mbar_wait(smem_u32(&ctl.r_full), done & 1, abort_flag, p.status, ASC_DEV_TIMEOUT_FULL);
         if (!ok) break;
@@ -477,6 +464,21 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
 }
 
+// CTAs [0, k_ctas) keep keys (dK, dV), the others queries (dQ)
+template <bool kBf16, int kHalves>
+__global__ void __launch_bounds__(kThreads, 1)
+    cross_bwd_kernel(const __grid_constant__ Maps k_maps, const __grid_constant__ Maps q_maps,
+                     const __grid_constant__ BwdParams pk, const __grid_constant__ BwdParams pq, const int k_ctas) {
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ BwdCtl ctl;
+  __shared__ Range range;
+  const int cta = blockIdx.x;
+  if (cta < k_ctas)
+    bwd_pass<kBf16, kHalves, true>(k_maps, pk, cta, k_ctas, smem_raw, ctl, range);
+  else
+    bwd_pass<kBf16, kHalves, false>(q_maps, pq, cta - k_ctas, gridDim.x - k_ctas, smem_raw, ctl, range);
+}
+
 template <bool kBf16>
 __device__ __forceinline__ float dot2(uint32_t a, uint32_t b) {
   if (kBf16)
@@ -485,68 +487,110 @@ __device__ __forceinline__ float dot2(uint32_t a, uint32_t b) {
   return x.x * y.x + x.y * y.y;
 }
 
-// -lse log2 e and -delta of every query row, a warp each; -inf and 0 for rows past the queries and rows without keys,
-// whose P is then 0.
+// -lse log2 e and -delta of every query row; -inf and 0 for rows past the queries and rows without keys, whose P is then
+// 0.  16 lanes a row (8 elements each), four rows of a lane loaded at once: HBM-bound on O and dO.
+constexpr int kRowsPerCta = 64;
 template <bool kBf16>
 __global__ void __launch_bounds__(256) cross_rows_kernel(const uint16_t* o, const uint16_t* dout, const float* lse,
-                                                         float* rows_l, float* rows_d, int64_t n, int Sq, int rows_pad, int Hq, int D,
-                                                         Strides os, Strides ds) {
-  const int lane = threadIdx.x & 31;
-  const int64_t i = blockIdx.x * 8ll + (threadIdx.x >> 5);
-  if (i >= n) return;
-  const int s = static_cast<int>(i % rows_pad);
-  const int64_t bh = i / rows_pad;
-  float2 r = make_float2(-INFINITY, 0.f);
-  if (s < Sq) {
-    const int64_t b = bh / Hq, h = bh % Hq;
-    float t = 0.f;
-    if (lane * 4 < D) {
-      const uint2 x = *reinterpret_cast<const uint2*>(o + b * os.b + s * os.s + h * os.h + lane * 4);
-      const uint2 y = *reinterpret_cast<const uint2*>(dout + b * ds.b + s * ds.s + h * ds.h + lane * 4);
-      t = dot2<kBf16>(x.x, y.x) + dot2<kBf16>(x.y, y.y);
-    }
+                                                         float* rows_l, float* rows_d, int64_t n, int Sq, int rows_pad,
+                                                         int Hq, int D, Strides os, Strides ds) {
+  const int lane = threadIdx.x & 15;
+  const int64_t i0 = static_cast<int64_t>(blockIdx.x) * kRowsPerCta + (threadIdx.x >> 4);
+  uint4 x[4], y[4];
+  float l[4];
 #pragma unroll
-    for (int k = 16; k > 0; k >>= 1) t += __shfl_xor_sync(0xffffffffu, t, k);
-    const float l = lse[bh * Sq + s];
-    if (l != -INFINITY) r = make_float2(-l * kLog2e, -t);
+  for (int k = 0; k < 4; ++k) {
+    const int64_t i = i0 + 16 * k;
+    x[k] = y[k] = make_uint4(0, 0, 0, 0);
+    l[k] = -INFINITY;
+    const int64_t bh = i / rows_pad;
+    const int s = static_cast<int>(i - bh * rows_pad);
+    if (i >= n || s >= Sq) continue;
+    const int64_t b = bh / Hq, h = bh - b * Hq;
+    if (lane * 8 < D) {
+      x[k] = *reinterpret_cast<const uint4*>(o + b * os.b + s * os.s + h * os.h + lane * 8);
+      y[k] = *reinterpret_cast<const uint4*>(dout + b * ds.b + s * ds.s + h * ds.h + lane * 8);
+    }
+    l[k] = lse[bh * Sq + s];
   }
-  if (elect_one()) rows_l[i] = r.x, rows_d[i] = r.y;
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    float t = dot2<kBf16>(x[k].x, y[k].x) + dot2<kBf16>(x[k].y, y[k].y) + dot2<kBf16>(x[k].z, y[k].z) + dot2<kBf16>(x[k].w, y[k].w);
+#pragma unroll
+    for (int m = 8; m > 0; m >>= 1) t += __shfl_xor_sync(0xffffffffu, t, m);
+    const int64_t i = i0 + 16 * k;
+    if (lane != 0 || i >= n) continue;
+    rows_l[i] = -l[k] * kLog2e, rows_d[i] = -t;
+    if (l[k] == -INFINITY) rows_l[i] = -INFINITY, rows_d[i] = 0.f;
+  }
 }
 
-// out[row] = scale * sum of the parts in order; rows of [B, S, H], a warp each
+// Adds the parts of a pass's cut items, in order: block column = border, D / 4 threads a row.
+template <bool kBf16, bool kKeys>
+__device__ __forceinline__ void add_parts(const BwdParams& p, int ctas) {
+  constexpr int kSums = kKeys ? 2 : 1, kRowsAtOnce = 4;
+  __shared__ ascsched::Cut cut;
+  __shared__ int found;
+  if (threadIdx.x < 32) {
+    ascsched::Cut mine;
+    const bool is = ascsched::find_cut(p.work, blockIdx.x + 1, ctas, mine);
+    if (threadIdx.x == 0) cut = mine, found = is;
+  }
+  __syncthreads();
+  if (!found) return;
+  const int per_row = p.D / 4, abreast = 256 / per_row;
+  const int c = threadIdx.x % per_row * 4, r0 = blockIdx.y * abreast * kRowsAtOnce + threadIdx.x / per_row;
+  if (threadIdx.x >= abreast * per_row) return;
+  float4 acc[kRowsAtOnce];
+#pragma unroll
+  for (int i = 0; i < kRowsAtOnce; ++i) acc[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+  cut.parts([&](int slot) {
+    float4 x[kRowsAtOnce];
+#pragma unroll
+    for (int i = 0; i < kRowsAtOnce; ++i) {
+      const int r = r0 + i * abreast;              // rows that do not exist were not written: they are not stored below
+      if (r < kSums * kTile)
+        x[i] = *reinterpret_cast<const float4*>(p.part + (static_cast<int64_t>(slot) * kSums * kTile + r) * p.D + c);
+    }
+#pragma unroll
+    for (int i = 0; i < kRowsAtOnce; ++i) acc[i].x += x[i].x, acc[i].y += x[i].y, acc[i].z += x[i].z, acc[i].w += x[i].w;
+  });
+#pragma unroll
+  for (int i = 0; i < kRowsAtOnce; ++i) {
+    const int r = r0 + i * abreast, w = r / kTile;
+    int s, h;
+    if (r >= kSums * kTile || !row_place<kKeys>(p, cut.item, r % kTile, s, h)) continue;
+    const float scale = w == 0 ? p.scale : 1.f;
+    if (kKeys && s >= cut.item.len) acc[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+    *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p.out[w]) + cut.item.b * p.ob[w] + s * p.os[w] + h * p.oh[w] + c) =
+        make_uint2(pack2<kBf16>(acc[i].x * scale, acc[i].y * scale), pack2<kBf16>(acc[i].z * scale, acc[i].w * scale));
+  }
+}
+
 template <bool kBf16>
-__global__ void __launch_bounds__(256) cross_add_kernel(const float* part, uint16_t* out, int64_t n, int splits, int S, int H,
-                                                        int D, Strides st, float scale) {
+__global__ void __launch_bounds__(256) cross_add_kernel(const BwdParams pk, const BwdParams pq, int k_ctas, int q_ctas) {
+  if (blockIdx.z == 0) {
+    if (pk.work.cut && blockIdx.x + 1 < k_ctas) add_parts<kBf16, true>(pk, k_ctas);
+  } else {
+    if (pq.work.cut && blockIdx.x + 1 < q_ctas) add_parts<kBf16, false>(pq, q_ctas);
+  }
+}
+
+// Zeros for a [B, S, H, D] gradient, a warp per row
+__global__ void __launch_bounds__(256) cross_zero_kernel(uint16_t* out, int64_t n, int S, int H, int D, Strides st) {
   const int c = (threadIdx.x & 31) * 4;
   const int64_t i = blockIdx.x * 8ll + (threadIdx.x >> 5);
   if (i >= n || c >= D) return;
-  float4 t = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int k = 0; k < splits; ++k) {
-    const float4 x = *reinterpret_cast<const float4*>(part + (k * n + i) * D + c);
-    t.x += x.x, t.y += x.y, t.z += x.z, t.w += x.w;
-  }
   const int64_t h = i % H, bs = i / H;
-  *reinterpret_cast<uint2*>(out + bs / S * st.b + bs % S * st.s + h * st.h + c) =
-      make_uint2(pack2<kBf16>(t.x * scale, t.y * scale), pack2<kBf16>(t.z * scale, t.w * scale));
+  *reinterpret_cast<uint2*>(out + bs / S * st.b + bs % S * st.s + h * st.h + c) = make_uint2(0u, 0u);
 }
 
 // ------------------------------------------------ host ---------------------------------------------------------
-// As in the forward, with a fixed cost of about six steps of 64 rows for an item (kept tiles, sums).
-int choose_splits(int64_t items, int64_t steps, int64_t sms) {
-  int best = 1;
-  int64_t best_cost = (items + sms - 1) / sms * (steps + 6);
-  for (int s = 2; s <= kMaxSplits && s <= steps; ++s) {
-    const int64_t cost = (items * s + sms - 1) / sms * ((steps + s - 1) / s + 6) + 8;
-    if (cost < best_cost) best_cost = cost, best = s;
-  }
-  return best;
-}
-
-template <bool kBf16, int kHalves, bool kKeys>
-int32_t launch_pass(const CUtensorMap& r1, const CUtensorMap& r2, const CUtensorMap& c1, const CUtensorMap& c2,
-                    const BwdParams& p, int sms, cudaStream_t stream) {
+template <bool kBf16, int kHalves>
+int32_t launch_bwd(const Maps& k_maps, const Maps& q_maps, const BwdParams& pk, const BwdParams& pq, int k_ctas, int q_ctas,
+                   cudaStream_t stream) {
   constexpr uint32_t smem = 2 * kHalves * kHalfTile + kStages * (2 * kHalves * kHalfStep + kStep * 8) + 1024;
-  auto kernel = cross_bwd_kernel<kBf16, kHalves, kKeys>;
+  auto kernel = cross_bwd_kernel<kBf16, kHalves>;
   static aschost::PerDevice attr_set;
   int dev = 0;
   ASC_CUDA_TRY(cudaGetDevice(&dev));
@@ -558,20 +602,19 @@ int32_t launch_pass(const CUtensorMap& r1, const CUtensorMap& r2, const CUtensor
     ASC_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
     attr_set.set(dev, 1);
   }
-  const uint32_t fmt = kBf16 ? 1u : 0u;
-  const uint32_t idesc_s = make_idesc(1, fmt, fmt, 0, 0, kTile, kKeys ? p.seg * p.pack : kStep);
-  const uint32_t idesc_acc = make_idesc(1, fmt, fmt, 0, 1, kTile, 64 * kHalves);
-  const int grid = p.items < sms ? p.items : sms;
-  kernel<<<grid, kThreads, smem, stream>>>(r1, r2, c1, c2, p, idesc_s, idesc_acc);
+  kernel<<<k_ctas + q_ctas, kThreads, smem, stream>>>(k_maps, q_maps, pk, pq, k_ctas);
   aschost::count_launch();
   ASC_CUDA_TRY(cudaGetLastError());
+  if (pk.work.cut || pq.work.cut) {
+    const int rows = 2 * kTile, per_cta = 256 / (pk.D / 4) * 4;
+    const int columns = (k_ctas > q_ctas ? k_ctas : q_ctas) - 1;
+    if (columns > 0) {
+      cross_add_kernel<kBf16><<<dim3(columns, (rows + per_cta - 1) / per_cta, 2), 256, 0, stream>>>(pk, pq, k_ctas, q_ctas);
+      aschost::count_launch();
+      ASC_CUDA_TRY(cudaGetLastError());
+    }
+  }
   return ASC_OK;
-}
-
-template <bool kBf16, bool kKeys>
-int32_t launch_any(const CUtensorMap* maps, const BwdParams& p, int sms, cudaStream_t st) {
-  return p.D <= 64 ? launch_pass<kBf16, 1, kKeys>(maps[0], maps[1], maps[2], maps[3], p, sms, st)
-                   : launch_pass<kBf16, 2, kKeys>(maps[0], maps[1], maps[2], maps[3], p, sms, st);
 }
 
 struct Call {
@@ -585,7 +628,7 @@ struct Call {
   cudaStream_t stream;
 };
 
-// Both passes on a workspace of `rows` (lse, delta) and, where a pass is cut, its parts.
+// Both passes, on a workspace of a -lse and a -delta per query row and, where items are cut, their parts.
 template <bool kBf16>
 int32_t run(const Call& c) {
   int sms = 0;
@@ -593,7 +636,6 @@ int32_t run(const Call& c) {
   if (rc != ASC_OK) return rc;
   const int64_t group = c.Hq / c.Hkv;
   BwdParams p{};
-  p.lengths = c.lengths;
   p.B = static_cast<int32_t>(c.B);
   p.Sq = static_cast<int32_t>(c.Sq);
   p.Skv = static_cast<int32_t>(c.Skv);
@@ -624,89 +666,82 @@ int32_t run(const Call& c) {
   pq.seg = pq.pack > 1 ? seg : kTile;
   pq.q_tiles_per_head = static_cast<int32_t>((c.Sq + kTile - 1) / kTile);
   const int64_t q_tiles = pq.pack > 1 ? (group + pq.pack - 1) / pq.pack : group * pq.q_tiles_per_head;
-  if (k_steps > (1 << 30) || c.B * c.Hkv * kv_tiles > 0x7fffffff / kMaxSplits ||
-      c.B * c.Hkv * q_tiles > 0x7fffffff / kMaxSplits || c.B * c.Hq > 0x7fffffff || c.B * c.Hq * rows_pad > (1ll << 33))
+  if (k_steps > (1 << 30) || c.B * c.Hkv * kv_tiles > 0x7fffffff || c.B * c.Hkv * q_tiles > 0x7fffffff ||
+      c.B * c.Hq > 0x7fffffff || c.B * c.Hq * rows_pad > (1ll << 33))
     return ASC_ERR_TOO_LARGE;
-  pk.q_tiles = static_cast<int32_t>(k_steps);
-  pk.kv_tiles = static_cast<int32_t>(kv_tiles);
-  pq.q_tiles = static_cast<int32_t>(q_tiles);
-  pk.splits = choose_splits(c.B * c.Hkv * kv_tiles, k_steps, sms);
-  pq.splits = choose_splits(c.B * c.Hkv * q_tiles, (c.Skv + kStep - 1) / kStep, sms);
-  pk.items = static_cast<int32_t>(c.B * c.Hkv * kv_tiles * pk.splits);
-  pq.items = static_cast<int32_t>(c.B * c.Hkv * q_tiles * pq.splits);
+  pk.work = {c.lengths, p.B, p.Skv, p.Hkv, static_cast<int32_t>(kv_tiles), static_cast<int32_t>(k_steps), kTile,
+             static_cast<int32_t>(c.B * c.Hkv * kv_tiles), 0, 0};
+  pq.work = {c.lengths, p.B, p.Skv, p.Hkv, static_cast<int32_t>(q_tiles), 0, kStep,
+             static_cast<int32_t>(c.B * c.Hkv * q_tiles), 0, 0};
+  // The passes share the SMs: each item an SM of its own where that is enough, otherwise by their products (a step has
+  // four for keys, three for queries, and what a step costs besides).
+  const int64_t q_steps = (c.Skv + kStep - 1) / kStep;
+  int k_sms = 0;
+  if (c.Skv > 0) {
+    const int64_t k_items = pk.work.items, q_items = pq.work.items;
+    const double k_cost = 6.0 * k_items * (k_steps + 5), q_cost = 5.0 * q_items * (q_steps + 5);
+    if (k_items + q_items <= sms) k_sms = static_cast<int>(k_items);
+    else k_sms = static_cast<int>(sms * k_cost / (k_cost + q_cost) + 0.5);
+    k_sms = k_sms < 1 ? 1 : k_sms > sms - 1 ? sms - 1 : k_sms;
+  }
+  // an item costs about five steps of 64 rows besides its own (kept tiles, sums), adding parts up about eight
+  const int k_grid = c.Skv > 0 ? ascsched::plan(pk.work, k_steps, k_sms, 2 * c.B * c.Sq * c.Hq * c.D * 2, 5, 8) : 0;
+  const int q_grid = ascsched::plan(pq.work, q_steps, sms - k_sms, 2 * c.B * c.Skv * c.Hkv * c.D * 2, 5, 8);
   pk.rows_pad = pq.rows_pad = static_cast<int32_t>(rows_pad);
 
-  // maps of each pass in its order: kept 1, kept 2, stream 1, stream 2
-  CUtensorMap mk[4], mq[4];
-  if (c.Skv > 0) {
-    if ((rc = encode_rows(&mk[0], kBf16, c.k, c.B, c.Skv, c.Hkv, c.D, c.sk, kTile, 1, &pk.k_heads, &pk.k_batches)) != ASC_OK ||
-        (rc = encode_rows(&mk[1], kBf16, c.v, c.B, c.Skv, c.Hkv, c.D, c.sv, kTile, 1, &pk.v_heads, &pk.v_batches)) != ASC_OK ||
-        (rc = encode_rows(&mk[2], kBf16, c.q, c.B, c.Sq, c.Hq, c.D, c.sq, pk.seg, pk.pack, nullptr, nullptr)) != ASC_OK ||
-        (rc = encode_rows(&mk[3], kBf16, c.dout, c.B, c.Sq, c.Hq, c.D, c.sdo, pk.seg, pk.pack, nullptr, nullptr)) != ASC_OK ||
-        (rc = encode_rows(&mq[2], kBf16, c.k, c.B, c.Skv, c.Hkv, c.D, c.sk, kStep, 1, &pq.k_heads, &pq.k_batches)) != ASC_OK ||
-        (rc = encode_rows(&mq[3], kBf16, c.v, c.B, c.Skv, c.Hkv, c.D, c.sv, kStep, 1, &pq.v_heads, &pq.v_batches)) != ASC_OK)
-      return rc;
-  }
-  if ((rc = encode_rows(&mq[0], kBf16, c.q, c.B, c.Sq, c.Hq, c.D, c.sq, pq.seg, pq.pack, nullptr, nullptr)) != ASC_OK ||
-      (rc = encode_rows(&mq[1], kBf16, c.dout, c.B, c.Sq, c.Hq, c.D, c.sdo, pq.seg, pq.pack, nullptr, nullptr)) != ASC_OK)
+  Maps mk, mq;
+  if ((rc = encode_rows(&mq.r1, kBf16, c.q, c.B, c.Sq, c.Hq, c.D, c.sq, pq.seg, pq.pack, nullptr, nullptr)) != ASC_OK ||
+      (rc = encode_rows(&mq.r2, kBf16, c.dout, c.B, c.Sq, c.Hq, c.D, c.sdo, pq.seg, pq.pack, nullptr, nullptr)) != ASC_OK)
     return rc;
-  if (c.Skv == 0) mq[2] = mq[3] = mq[0];        // never read: no item has a step
+  if (c.Skv == 0) {
+    mq.c1 = mq.c2 = mq.r1;        // never read: no item has a step
+    mk = mq;
+  } else if ((rc = encode_rows(&mk.r1, kBf16, c.k, c.B, c.Skv, c.Hkv, c.D, c.sk, kTile, 1, &pk.k_heads, &pk.k_batches)) != ASC_OK ||
+             (rc = encode_rows(&mk.r2, kBf16, c.v, c.B, c.Skv, c.Hkv, c.D, c.sv, kTile, 1, &pk.v_heads, &pk.v_batches)) != ASC_OK ||
+             (rc = encode_rows(&mk.c1, kBf16, c.q, c.B, c.Sq, c.Hq, c.D, c.sq, pk.seg, pk.pack, nullptr, nullptr)) != ASC_OK ||
+             (rc = encode_rows(&mk.c2, kBf16, c.dout, c.B, c.Sq, c.Hq, c.D, c.sdo, pk.seg, pk.pack, nullptr, nullptr)) != ASC_OK ||
+             (rc = encode_rows(&mq.c1, kBf16, c.k, c.B, c.Skv, c.Hkv, c.D, c.sk, kStep, 1, &pq.k_heads, &pq.k_batches)) != ASC_OK ||
+             (rc = encode_rows(&mq.c2, kBf16, c.v, c.B, c.Skv, c.Hkv, c.D, c.sv, kStep, 1, &pq.v_heads, &pq.v_batches)) != ASC_OK) {
+    return rc;
+  }
 
   const size_t n_rows = static_cast<size_t>(c.B) * c.Hq * rows_pad;
-  const size_t n_q = static_cast<size_t>(c.B) * c.Sq * c.Hq, n_k = static_cast<size_t>(c.B) * c.Skv * c.Hkv;
-  const size_t rows_bytes = (n_rows * 2 * sizeof(float) + 255) / 256 * 256;
-  const size_t q_bytes = pq.splits > 1 ? pq.splits * n_q * c.D * sizeof(float) : 0;
-  const size_t k_bytes = pk.splits > 1 ? pk.splits * n_k * c.D * sizeof(float) : 0;
+  const size_t rows_bytes = (n_rows * 2 * sizeof(float) + 255) / 256 * 256, slot_bytes = static_cast<size_t>(kTile) * c.D * sizeof(float);
+  const size_t k_bytes = pk.work.cut ? 4 * k_grid * slot_bytes : 0, q_bytes = pq.work.cut ? 2 * q_grid * slot_bytes : 0;
   void* ws = nullptr;
-  if ((rc = aschost::scratch_alloc(&ws, rows_bytes + q_bytes + 2 * k_bytes, c.stream)) != ASC_OK) return rc;
+  if ((rc = aschost::scratch_alloc(&ws, rows_bytes + k_bytes + q_bytes, c.stream)) != ASC_OK) return rc;
   char* at = static_cast<char*>(ws);
   float* rows = reinterpret_cast<float*>(at);
   pk.rows_l = pq.rows_l = rows;
   pk.rows_d = pq.rows_d = rows + n_rows;
-  pq.part[0] = reinterpret_cast<float*>(at + rows_bytes);
-  pk.part[0] = reinterpret_cast<float*>(at + rows_bytes + q_bytes);
-  pk.part[1] = reinterpret_cast<float*>(at + rows_bytes + q_bytes + k_bytes);
+  pk.part = reinterpret_cast<float*>(at + rows_bytes);
+  pq.part = reinterpret_cast<float*>(at + rows_bytes + k_bytes);
   for (int i = 0; i < 3; ++i) {
     BwdParams& to = i == 0 ? pq : pk;
     const int w = i == 2;
     to.out[w] = c.grad[i];
     to.ob[w] = c.sg[i].b, to.os[w] = c.sg[i].s, to.oh[w] = c.sg[i].h;
   }
-  auto finish = [&](cudaError_t e, const char* what) {
-    if (e != cudaSuccess) return aschost::record_cuda_error(e, what);
-    aschost::count_launch();
-    return static_cast<int32_t>(ASC_OK);
-  };
-  auto add = [&](const float* part, int i, int64_t n, int splits, int64_t S, int64_t H, float scale) {
-    cross_add_kernel<kBf16><<<static_cast<unsigned>((n + 7) / 8), 256, 0, c.stream>>>(
-        part, static_cast<uint16_t*>(c.grad[i]), n, splits, static_cast<int>(S), static_cast<int>(H), static_cast<int>(c.D),
-        c.sg[i], scale);
-    return finish(cudaGetLastError(), "cross_add_kernel");
-  };
-  cross_rows_kernel<kBf16><<<static_cast<unsigned>((n_rows + 7) / 8), 256, 0, c.stream>>>(
+  cross_rows_kernel<kBf16><<<static_cast<unsigned>((n_rows + kRowsPerCta - 1) / kRowsPerCta), 256, 0, c.stream>>>(
       static_cast<const uint16_t*>(c.o), static_cast<const uint16_t*>(c.dout), c.lse, rows, rows + n_rows,
       static_cast<int64_t>(n_rows), p.Sq, pk.rows_pad, static_cast<int>(c.Hq), p.D, c.so, c.sdo);
-  rc = finish(cudaGetLastError(), "cross_rows_kernel");
-  if (rc == ASC_OK && c.Skv > 0) rc = launch_any<kBf16, true>(mk, pk, sms, c.stream);
-  if (rc == ASC_OK) rc = launch_any<kBf16, false>(mq, pq, sms, c.stream);
-  if (rc == ASC_OK && pk.splits > 1) {
-    rc = add(pk.part[0], 1, n_k, pk.splits, c.Skv, c.Hkv, c.scale);
-    if (rc == ASC_OK) rc = add(pk.part[1], 2, n_k, pk.splits, c.Skv, c.Hkv, 1.f);
-  }
-  if (rc == ASC_OK && pq.splits > 1) rc = add(pq.part[0], 0, n_q, pq.splits, c.Sq, c.Hq, c.scale);
+  const cudaError_t e = cudaGetLastError();
+  if (e == cudaSuccess) aschost::count_launch();
+  else rc = aschost::record_cuda_error(e, "cross_rows_kernel");
+  if (rc == ASC_OK)
+    rc = c.D <= 64 ? launch_bwd<kBf16, 1>(mk, mq, pk, pq, k_grid, q_grid, c.stream)
+                   : launch_bwd<kBf16, 2>(mk, mq, pk, pq, k_grid, q_grid, c.stream);
   const int32_t freed = aschost::scratch_free(ws, c.stream);
   return rc == ASC_OK ? freed : rc;
 }
 
 // Without a query the gradients of k and v are sums of nothing.
-template <bool kBf16>
 int32_t no_queries(const Call& c) {
   const int64_t n = c.B * c.Skv * c.Hkv;
   if ((n + 7) / 8 > 0x7fffffff) return ASC_ERR_TOO_LARGE;
   for (int i = 1; i < 3; ++i) {
-    cross_add_kernel<kBf16><<<static_cast<unsigned>((n + 7) / 8), 256, 0, c.stream>>>(
-        nullptr, static_cast<uint16_t*>(c.grad[i]), n, 0, static_cast<int>(c.Skv), static_cast<int>(c.Hkv),
-        static_cast<int>(c.D), c.sg[i], 1.f);
+    cross_zero_kernel<<<static_cast<unsigned>((n + 7) / 8), 256, 0, c.stream>>>(
+        static_cast<uint16_t*>(c.grad[i]), n, static_cast<int>(c.Skv), static_cast<int>(c.Hkv), static_cast<int>(c.D), c.sg[i]);
     ASC_CUDA_TRY(cudaGetLastError());
     aschost::count_launch();
   }
@@ -742,7 +777,7 @@ extern "C" int32_t asc_cuda_cross_attn_bwd_f16(const void* d_o, const void* q, c
       if ((rc = check_operand(v, c.sv, c.B, c.Skv, c.Hkv, false)) != ASC_OK) return rc;
     }
   }
-  if (!queries) return dtype == 1 ? no_queries<true>(c) : no_queries<false>(c);
+  if (!queries) return no_queries(c);
   // (queries and their gradients must not repeat memory; see the forward)
   if ((rc = check_operand(q, c.sq, c.B, c.Sq, c.Hq, true)) != ASC_OK) return rc;
   if ((rc = check_operand(d_o, c.sdo, c.B, c.Sq, c.Hq, true)) != ASC_OK) return rc;
