@@ -114,6 +114,7 @@ __device__ __forceinline__ void find_range(const Schedule& s, int cta, int ctas,
 struct Walker {
   int cta, ctas, u, pos, end, start, b, base, tiles, steps, len;
 
+  Walker() = default;
   __device__ Walker(const Schedule& s, const Range& r, int cta_, int ctas_)
       : cta(cta_), ctas(ctas_), u(cta_), pos(r.pos), end(r.end), start(r.pos), b(r.b), base(r.base) {
     if (pos < end) load(s);
@@ -151,6 +152,31 @@ struct Walker {
     g.slot = g.n == steps ? -1 : 2 * cta + (pos != start);
     pos += g.n;
     return true;
+  }
+};
+
+// A warp's walk kept in shared memory, for the warps whose registers are full of scores: `next` puts the segment there
+// too.  Called by whole warps, each with a Walk of its own.
+struct Walk {
+  Walker walker;
+  Segment segment;
+
+  __device__ void start(const Schedule& s, const Range& r, int cta, int ctas) {
+    const Walker w(s, r, cta, ctas);
+    if ((threadIdx.x & 31) == 0) walker = w;
+    __syncwarp();
+  }
+  __device__ bool next(const Schedule& s) {
+    Walker w = walker;
+    Segment g;
+    const bool more = w.next(s, g);
+    __syncwarp();
+    if ((threadIdx.x & 31) == 0) {
+      walker = w;
+      if (more) segment = g;
+    }
+    __syncwarp();
+    return more;
   }
 };
 

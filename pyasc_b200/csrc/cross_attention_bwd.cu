@@ -183,7 +183,7 @@ struct Maps {
 
 template <bool kBf16, int kHalves, bool kKeys>
 __device__ __forceinline__ void bwd_pass(const Maps& maps, const BwdParams& p, const int cta, const int ctas,
-                                         uint8_t* smem_raw, BwdCtl& ctl, Range& range) {
+                                         uint8_t* smem_raw, BwdCtl& ctl, Range& range, ascsched::Walk* walks) {
   const CUtensorMap &tmap_r1 = maps.r1, &tmap_r2 = maps.r2, &tmap_c1 = maps.c1, &tmap_c2 = maps.c2;
   constexpr uint32_t kFmt = kBf16 ? 1u : 0u;
   const uint32_t idesc_s = make_idesc(1, kFmt, kFmt, 0, 0, kTile, kKeys ? p.seg * p.pack : kStep);
@@ -254,16 +254,19 @@ __device__ __forceinline__ void bwd_pass(const Maps& maps, const BwdParams& p, c
         write_row<kBf16, 16 * kHalves>(p, t_base + kColAcc + col0, 0, col0, valid, it.n == 0, gone, it.b, s, h, part, p.scale);
       }
     };
-    Walker walk(p.work, range, cta, ctas);
-    Segment it;
-    while (ok && walk.next(p.work, it)) {
+    ascsched::Walk& walk = walks[warp];
+    walk.start(p.work, range, cta, ctas);
+    const Segment& it = walk.segment;
+    while (ok && walk.next(p.work)) {
+      const int steps = it.n;
+      int limit = it.len - 1 - it.first * kStep - half * 32;
       int s, h;
       float neg_l = 0.f, neg_d = 0.f;
       if (!kKeys && row_place<kKeys>(p, it, row, s, h)) {
         const int64_t at = (static_cast<int64_t>(it.b) * (p.Hkv * p.group) + h) * p.rows_pad + s;
         neg_l = p.rows_l[at], neg_d = p.rows_d[at];
       }
-      for (int i = 0; i < it.n && ok; ++i) {
+      for (int i = 0; i < steps && ok; ++i, limit -= kStep) {
         const uint32_t step = g + i, buf = step & 1;
         if (static_cast<int>(buf) != parity) continue;
         if (kKeys) {           // the rows' lse and delta were written by the copy that this barrier counts
@@ -275,15 +278,15 @@ __device__ __forceinline__ void bwd_pass(const Maps& maps, const BwdParams& p, c
         tc_fence_after();
         const float* cols = reinterpret_cast<const float*>(pairs + (step % kStages) * (kStep * 8));
         step_math<kBf16, kKeys>(t_base + kColS + buf * 128 + half * 32, cols, cols + kStep, neg_l, neg_d, p.scale_log2,
-                                kKeys ? 0 : it.len - 1 - (it.first + i) * kStep - half * 32);
+                                limit);
         tmem_st_wait();
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(smem_u32(&ctl.p_full[buf]));
       }
       if (!ok) break;
-      g += it.n;
-      const bool zero = it.n == 0;
+      g += steps;
+      const bool zero = steps == 0;
       if (!zero) {
         ok = mbar_wait(smem_u32(&ctl.acc_full), done & 1, abort_flag, p.status, ASC_DEV_TIMEOUT_TMEM_FULL);
         if (!ok) break;
@@ -472,11 +475,12 @@ __global__ void __launch_bounds__(kThreads, 1)
   extern __shared__ uint8_t smem_raw[];
   __shared__ BwdCtl ctl;
   __shared__ Range range;
+  __shared__ ascsched::Walk walks[kMathWarps];
   const int cta = blockIdx.x;
   if (cta < k_ctas)
-    bwd_pass<kBf16, kHalves, true>(k_maps, pk, cta, k_ctas, smem_raw, ctl, range);
+    bwd_pass<kBf16, kHalves, true>(k_maps, pk, cta, k_ctas, smem_raw, ctl, range, walks);
   else
-    bwd_pass<kBf16, kHalves, false>(q_maps, pq, cta - k_ctas, gridDim.x - k_ctas, smem_raw, ctl, range);
+    bwd_pass<kBf16, kHalves, false>(q_maps, pq, cta - k_ctas, gridDim.x - k_ctas, smem_raw, ctl, range, walks);
 }
 
 template <bool kBf16>
