@@ -23,6 +23,7 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
 constexpr int kMaxHeadDim = 1024;
+constexpr int kFwdCtas = 3;     // per SM: 80 registers a thread (2: 74, 3: 67, 4, which spills: 86 us at [1, 16384, 32 + 8, 128])
 
 struct Operand {           // a [batch, sequence, head, dim] tensor: strides in elements, dim contiguous
   void* p;
@@ -258,48 +259,57 @@ __device__ __forceinline__ float2* stage(const RotaryArgs& a, float* smem) {
   return reinterpret_cast<float2*>(smem + floats) + (threadIdx.x >> 5) * (a.r / 2);
 }
 
+// What a group of lanes does next: rows of one token, queries (w = 0) and then keys, each from head `first` in steps.
+struct Place {
+  int b, s, first;
+};
+
+// The vectors of one tensor's rows that a lane owns, as a pointer that walks over the heads of a token.
+template <typename T>
+struct RowWalk {
+  const uint4* at;
+  int64_t stride;            // in 16-byte vectors
+  __device__ RowWalk(const Operand& o, const Place& p, int v0, int step)
+      : at(reinterpret_cast<const uint4*>(row_of<const T>(o, p.b, p.s, p.first)) + v0), stride(o.h * step / Vec<T>::E) {}
+  __device__ void next() { at += stride; }
+  __device__ uint4* out() const { return const_cast<uint4*>(at); }
+};
+
 // --------------------------------------------------------------------------------------------------------------
 // Forward, whole 16-byte vectors.  A warp works on one token, or on a slice of its heads where tokens are few: it
 // computes the token's angles into its own piece of shared memory (no barrier beyond the warp), then its groups of
-// lanes take the heads in turn, queries first and then keys.  The next row, also the next token's first, is loaded
-// before the current one is computed.  Warps stride over the tokens.
+// lanes take the queries in turn and then the keys.  The next row, also the next token's first, is loaded before the
+// current one is computed.  Warps stride over the tokens.
 // --------------------------------------------------------------------------------------------------------------
 template <typename T, bool kNorm, bool kInter>
-__global__ void __launch_bounds__(kThreads) rotary_fwd_kernel(const RotaryArgs a) {
+__global__ void __launch_bounds__(kThreads, kFwdCtas) rotary_fwd_kernel(const __grid_constant__ RotaryArgs a) {
   constexpr int E = Vec<T>::E;
   extern __shared__ float smem[];
   float2* table = stage(a, smem);
   const int lane = threadIdx.x & ((1 << a.log_lanes) - 1), group = (threadIdx.x & 31) >> a.log_lanes;
   const int groups = 32 >> a.log_lanes;
-  const int H = a.heads[0] + a.heads[1];
   const int step = groups * a.slices;
-  const int iters = (H + step - 1) / step;
   const int warps = gridDim.x * kWarps;
   const int units = a.tokens * a.slices;
   const LaneVectors<E> l(a, lane);
   const float inv_d = 1.f / a.D;
+  const int w_first = a.heads[0] > 0 ? 0 : 1;
 
-  struct Place {
-    int b, s, first;       // token and first head of this group
-  };
   auto place = [&](int unit) {
     const int token = unit / a.slices;
     const int b = token / a.S;
     return Place{b, token - b * a.S, (unit - token * a.slices) * groups + group};
   };
-  auto load = [&](const Place& p, int h, uint4& lo, uint4& hi) {
+  auto load = [&](const uint4* at, bool on, uint4& lo, uint4& hi) {
     lo = hi = make_uint4(0, 0, 0, 0);
-    if (h >= H) return;
-    const int w = h >= a.heads[0];
-    const uint4* row = reinterpret_cast<const uint4*>(row_of<const T>(a.x[w], p.b, p.s, h - (w ? a.heads[0] : 0)));
-    if (l.has0) lo = row[l.v0];
-    if (l.has1) hi = row[l.v1];
+    if (on && l.has0) lo = at[0];
+    if (on && l.has1) hi = at[l.v1 - l.v0];
   };
   int unit = blockIdx.x * kWarps + (threadIdx.x >> 5);
   if (unit >= units) return;
   Place p = place(unit);
   uint4 lo, hi;
-  load(p, p.first, lo, hi);
+  load(RowWalk<T>(a.x[w_first], p, l.v0, step).at, p.first < a.heads[w_first], lo, hi);
   double pos = a.r > 0 ? position_at(a, p.b, p.s) : 0.0;
   for (; unit < units; unit += warps) {
     __syncwarp();                                  // the previous token's angles are no longer read
@@ -312,32 +322,42 @@ __global__ void __launch_bounds__(kThreads) rotary_fwd_kernel(const RotaryArgs a
       if (a.r > 0) pos = position_at(a, next.b, next.s);
     }
     Turn<E> t;
-    int which = -1;
-    for (int it = 0; it < iters; ++it) {
-      const int h = p.first + it * step;
-      const int w = h >= a.heads[0];
-      float2 v[E];
-      Vec<T>::unpack(lo, reinterpret_cast<float*>(v));
-      Vec<T>::unpack(hi, reinterpret_cast<float*>(v + E / 2));
-      if (it + 1 < iters) load(p, h + step, lo, hi);
-      else if (more) load(next, next.first, lo, hi);
-      if (kNorm ? w != which : which < 0) {
-        which = w;
-        lane_turn<E, kInter, kNorm>(a, l, table, smem + w * a.D, t);
-      }
-      if (kNorm) {
-        float2 ss = make_float2(0.f, 0.f);
+    if (!kNorm) lane_turn<E, kInter, kNorm>(a, l, table, nullptr, t);
+#pragma unroll 1
+    for (int w = 0; w < 2; ++w) {
+      const int H = a.heads[w];
+      if (H == 0) continue;
+      const int iters = (H + step - 1) / step;
+      if (kNorm) lane_turn<E, kInter, kNorm>(a, l, table, smem + w * a.D, t);
+      RowWalk<T> in(a.x[w], p, l.v0, step), out(a.y[w], p, l.v0, step);
+      int h = p.first;
+      for (int it = 0; it < iters; ++it, h += step) {
+        float2 v[E];
+        Vec<T>::unpack(lo, reinterpret_cast<float*>(v));
+        Vec<T>::unpack(hi, reinterpret_cast<float*>(v + E / 2));
+        if (it + 1 < iters) {
+          in.next();
+          load(in.at, h + step < H, lo, hi);
+        } else if (w == 0 && a.heads[1] > 0) {
+          load(RowWalk<T>(a.x[1], p, l.v0, step).at, p.first < a.heads[1], lo, hi);
+        } else if (more) {
+          load(RowWalk<T>(a.x[w_first], next, l.v0, step).at, next.first < a.heads[w_first], lo, hi);
+        }
+        if (kNorm) {
+          float2 ss = make_float2(0.f, 0.f);
 #pragma unroll
-        for (int e = 0; e < E; ++e) ss = __ffma2_rn(v[e], v[e], ss);
-        const float rstd = rsqrtf(group_sum(ss.x + ss.y, a.log_lanes) * inv_d + a.eps);
+          for (int e = 0; e < E; ++e) ss = __ffma2_rn(v[e], v[e], ss);
+          const float rstd = rsqrtf(group_sum(ss.x + ss.y, a.log_lanes) * inv_d + a.eps);
 #pragma unroll
-        for (int e = 0; e < E; ++e) v[e] = __fmul2_rn(v[e], make_float2(rstd, rstd));
-      }
-      if (h < H) {
-        apply<E, kInter>(a, l, t, v);
-        uint4* row = reinterpret_cast<uint4*>(row_of<T>(a.y[w], p.b, p.s, h - (w ? a.heads[0] : 0)));
-        if (l.has0) row[l.v0] = Vec<T>::pack(reinterpret_cast<float*>(v));
-        if (l.has1) row[l.v1] = Vec<T>::pack(reinterpret_cast<float*>(v + E / 2));
+          for (int e = 0; e < E; ++e) v[e] = __fmul2_rn(v[e], make_float2(rstd, rstd));
+        }
+        if (h < H) {
+          apply<E, kInter>(a, l, t, v);
+          uint4* row = out.out();
+          if (l.has0) row[0] = Vec<T>::pack(reinterpret_cast<float*>(v));
+          if (l.has1) row[l.v1 - l.v0] = Vec<T>::pack(reinterpret_cast<float*>(v + E / 2));
+        }
+        out.next();
       }
     }
     p = next;
@@ -350,7 +370,7 @@ __global__ void __launch_bounds__(kThreads) rotary_fwd_kernel(const RotaryArgs a
 // after them, so that queries and keys share the angles without two sets of sums in registers.
 // --------------------------------------------------------------------------------------------------------------
 template <typename T, bool kInter>
-__global__ void __launch_bounds__(kThreads, 2) rotary_bwd_kernel(const RotaryArgs a) {
+__global__ void __launch_bounds__(kThreads, 2) rotary_bwd_kernel(const __grid_constant__ RotaryArgs a) {
   constexpr int E = Vec<T>::E;
   extern __shared__ float smem[];
   float2* table = stage(a, smem);
@@ -368,9 +388,6 @@ __global__ void __launch_bounds__(kThreads, 2) rotary_bwd_kernel(const RotaryArg
 #pragma unroll
   for (int e = 0; e < 2 * E; ++e) sums[e * kThreads + threadIdx.x] = make_float2(0.f, 0.f);
 
-  struct Place {
-    int b, s, first;
-  };
   auto place = [&](int unit) {
     const int token = unit / a.slices;
     const int b = token / a.S;
@@ -744,8 +761,8 @@ int32_t launch_fwd(RotaryArgs a, const Problem& pr, cudaStream_t st) {
     rotary_any_kernel<T, false><<<static_cast<unsigned>(grid), kThreads, a.r / 2 * sizeof(float2), st>>>(a);
   } else {
     a.log_lanes = log2_of(lanes);
-    a.slices = slices_for(tokens, H, 32 / lanes, 16ll * sms);
-    const int64_t units = tokens * a.slices, most = 2ll * sms;
+    a.slices = slices_for(tokens, a.heads[0] > a.heads[1] ? a.heads[0] : a.heads[1], 32 / lanes, static_cast<int64_t>(kFwdCtas) * kWarps * sms);
+    const int64_t units = tokens * a.slices, most = static_cast<int64_t>(kFwdCtas) * sms;
     const unsigned grid = static_cast<unsigned>(units < most * kWarps ? (units + kWarps - 1) / kWarps : most);
     const size_t smem = vector_smem(a);
     if (a.norm) {
