@@ -732,13 +732,14 @@ int log2_of(int64_t v) {
   return l;
 }
 
-// Parts of a token's heads: one, unless the tokens are fewer than four for each warp that can be resident (a second
-// part costs the token's angles once more, an idle warp more than that).  No part has less than one row for a group.
-int32_t slices_for(int64_t tokens, int64_t heads, int64_t groups, int64_t warps) {
+// Parts of a token's heads: one, unless the tokens leave warps idle; then a power of two up to `rounds` parts for each
+// warp that can be resident.  A part costs the token's angles (and gammas) once more.  No part has less than one row for
+// a group.
+int32_t slices_for(int64_t tokens, int64_t heads, int64_t groups, int64_t warps, int64_t rounds) {
   const int64_t most = (heads + groups - 1) / groups;
-  int64_t slices = (4 * warps + tokens - 1) / tokens;
-  if (slices > most) slices = most;
-  return static_cast<int32_t>(slices < 1 ? 1 : slices);
+  int64_t slices = 1;
+  while (2 * slices <= most && tokens * slices < rounds * warps) slices *= 2;
+  return static_cast<int32_t>(slices);
 }
 
 size_t vector_smem(const RotaryArgs& a) {
@@ -752,7 +753,6 @@ int32_t launch_fwd(RotaryArgs a, const Problem& pr, cudaStream_t st) {
   if (rc != ASC_OK) return rc;
   constexpr int E = Vec<T>::E;
   const int64_t tokens = a.tokens;
-  const int H = a.heads[0] + a.heads[1];
   int lanes = vector_lanes(pr, a.interleaved);
   for (int w = 0; w < 2; ++w)
     if (pr.H[w] > 0 && !(is_vector_operand(a.x[w], E) && is_vector_operand(a.y[w], E))) lanes = 0;
@@ -761,7 +761,7 @@ int32_t launch_fwd(RotaryArgs a, const Problem& pr, cudaStream_t st) {
     rotary_any_kernel<T, false><<<static_cast<unsigned>(grid), kThreads, a.r / 2 * sizeof(float2), st>>>(a);
   } else {
     a.log_lanes = log2_of(lanes);
-    a.slices = slices_for(tokens, a.heads[0] > a.heads[1] ? a.heads[0] : a.heads[1], 32 / lanes, static_cast<int64_t>(kFwdCtas) * kWarps * sms);
+    a.slices = slices_for(tokens, a.heads[0] > a.heads[1] ? a.heads[0] : a.heads[1], 32 / lanes, static_cast<int64_t>(kFwdCtas) * kWarps * sms, 2);
     const int64_t units = tokens * a.slices, most = static_cast<int64_t>(kFwdCtas) * sms;
     const unsigned grid = static_cast<unsigned>(units < most * kWarps ? (units + kWarps - 1) / kWarps : most);
     const size_t smem = vector_smem(a);
@@ -794,7 +794,7 @@ int32_t launch_bwd(RotaryArgs a, const Problem& pr, float* dq_gamma, float* dk_g
   int64_t rows[2];             // rows of partial sums of the gammas, queries' first
   if (lanes != 0) {
     a.log_lanes = log2_of(lanes);
-    a.slices = slices_for(a.tokens, H, 32 / lanes, 8ll * slots);
+    a.slices = slices_for(a.tokens, H, 32 / lanes, kWarps * slots, 1);
     const int64_t units = static_cast<int64_t>(a.tokens) * a.slices;
     rows[0] = rows[1] = units < slots * kWarps ? (units + kWarps - 1) / kWarps : slots;
   } else {
