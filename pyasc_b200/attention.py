@@ -13,7 +13,7 @@ from __future__ import annotations
 
 import math
 import struct
-from typing import Optional, Sequence, Tuple
+from typing import Dict, Optional, Sequence, Tuple
 
 import torch
 
@@ -25,8 +25,24 @@ _DTYPE_CODE = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}
 # --------------------------------------------------------------------------------------------------
 # Arguments
 # --------------------------------------------------------------------------------------------------
-# A call's host time is a large part of the smallest launches: the checks read each property of a tensor once and
-# leave the wording of an error to the second look.
+# A call's host time is most of the smallest launches, and a program makes the same call over and over: what the checks
+# allow, and the sizes and strides they pack for the C ABI, are kept by the arguments' layouts (shapes, strides, types,
+# device; never addresses or contents).
+_layouts: Dict[tuple, tuple] = {}
+_MAX_LAYOUTS = 1024
+
+
+def _layout(t: Optional[torch.Tensor]):
+    return None if t is None else (t.shape, t.stride(), t.dtype, t.get_device())
+
+
+def _remember(key: tuple, plan: tuple) -> tuple:
+    if len(_layouts) >= _MAX_LAYOUTS:
+        _layouts.clear()
+    _layouts[key] = plan
+    return plan
+
+
 def _device_of(name: str, t: torch.Tensor) -> int:
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{name} must be a torch tensor, got {type(t).__name__}")
@@ -79,7 +95,7 @@ _NO_STRIDES = (0, 0, 0)
 def _call(fn_name: str, device: int, *args) -> None:
     """One C-ABI call with ``device`` current, on its current torch stream."""
     stream = torch._C._cuda_getCurrentRawStream(device)
-    if device == torch.cuda.current_device():
+    if device == torch._C._cuda_getDevice():
         capi.call(fn_name, *args, stream)
     else:
         with torch.cuda.device(device):
@@ -182,17 +198,35 @@ def _gammas(device: int, head_dim: int, q_gamma: Optional[torch.Tensor], k_gamma
     return code or 0
 
 
-def _rotate(q, k, q_gamma, k_gamma, positions, frequencies, eps, scale, interleaved, flags, q_out, k_out):
+def _rotary_plan(tensors, interleaved, flags):
+    """Checks of a forward call: device, codes of the types, flags, dims, and strides but for those of the outputs."""
+    q, k, q_gamma, k_gamma, positions, frequencies, q_out, k_out = tensors
     device, q_shape, k_shape, dims, pos_strides, pos_flag = _rotary_arguments(q, k, positions, frequencies)
     if k is None and (k_out is not None or k_gamma is not None):
         raise ValueError("an output or a gamma of k without k")
-    gamma_code = 0 if q_gamma is None and k_gamma is None else _gammas(device, q_shape[3], q_gamma, k_gamma)
+    gamma_code = _gammas(device, q_shape[3], q_gamma, k_gamma)
     q_out = _output("the output of q", q_out, q, q_shape, device)
     k_out = None if k is None else _output("the output of k", k_out, k, k_shape, device)
+    strides = _PACK[14](*_strides(q), *_strides(k), *_strides(q_out), *_strides(k_out), *pos_strides)
+    return device, dims, strides, _DTYPE_CODE[q.dtype], gamma_code, flags | pos_flag | bool(interleaved)
+
+
+def _rotate(q, k, q_gamma, k_gamma, positions, frequencies, eps, scale, interleaved, flags, q_out, k_out):
+    tensors = (q, k, q_gamma, k_gamma, positions, frequencies, q_out, k_out)
+    try:
+        key = (flags, interleaved, *map(_layout, tensors))
+        plan = _layouts.get(key)
+    except AttributeError:               # not tensors: the checks say which
+        key = plan = None
+    if plan is None:
+        plan = _remember(key, _rotary_plan(tensors, interleaved, flags))
+    device, dims, strides, code, gamma_code, flags = plan
+    if q_out is None:
+        q_out = torch.empty_like(q)
+    if k_out is None and k is not None:
+        k_out = torch.empty_like(k)
     _call("asc_cuda_norm_rotary", device, q.data_ptr(), _ptr(k), q_out.data_ptr(), _ptr(k_out), _ptr(q_gamma),
-          _ptr(k_gamma), positions.data_ptr(), frequencies.data_ptr(), dims,
-          _PACK[14](*_strides(q), *_strides(k), *_strides(q_out), *_strides(k_out), *pos_strides), eps, scale,
-          _DTYPE_CODE[q.dtype], gamma_code, flags | pos_flag | bool(interleaved))
+          _ptr(k_gamma), positions.data_ptr(), frequencies.data_ptr(), dims, strides, eps, scale, code, gamma_code, flags)
     return q_out, k_out
 
 
@@ -227,13 +261,8 @@ def norm_rotary(q: torch.Tensor, k: Optional[torch.Tensor], q_gamma: Optional[to
     return _rotate(q, k, q_gamma, k_gamma, positions, frequencies, eps, scale, interleaved, 2, q_out, k_out)
 
 
-def norm_rotary_backward(dq_out: torch.Tensor, dk_out: Optional[torch.Tensor], q: torch.Tensor, k: Optional[torch.Tensor],
-                         q_gamma: Optional[torch.Tensor], k_gamma: Optional[torch.Tensor], positions: torch.Tensor,
-                         frequencies: torch.Tensor, *, eps: float = 1e-6, scale: float = 1.0, interleaved: bool = False,
-                         dq: Optional[torch.Tensor] = None, dk: Optional[torch.Tensor] = None):
-    """Gradients ``(dq, dk, dq_gamma, dk_gamma)`` of :func:`norm_rotary` from those of its outputs and its inputs.  The
-    gammas' gradients are float32 sums over all rows in a fixed order (None where there is no gamma).  ``dq`` may be
-    ``dq_out`` or ``q``, ``dk`` likewise."""
+def _rotary_backward_plan(tensors, interleaved):
+    dq_out, dk_out, q, k, q_gamma, k_gamma, positions, frequencies, dq, dk = tensors
     device, q_shape, k_shape, dims, pos_strides, pos_flag = _rotary_arguments(q, k, positions, frequencies)
     if (k is None) != (dk_out is None):
         raise ValueError("k and dk_out go together")
@@ -245,20 +274,43 @@ def norm_rotary_backward(dq_out: torch.Tensor, dk_out: Optional[torch.Tensor], q
     if k is not None:
         _check_shape("dk_out", _check_rows("dk_out", dk_out, q.dtype, device), k_shape)
         dk = _output("dk", dk, k, k_shape, device)
+    strides = _PACK[20](*_strides(dq_out), *_strides(dk_out), *_strides(q), *_strides(k), *_strides(dq), *_strides(dk),
+                        *pos_strides)
+    return device, dims, strides, _DTYPE_CODE[q.dtype], gamma_code, 2 | pos_flag | bool(interleaved)
+
+
+def norm_rotary_backward(dq_out: torch.Tensor, dk_out: Optional[torch.Tensor], q: torch.Tensor, k: Optional[torch.Tensor],
+                         q_gamma: Optional[torch.Tensor], k_gamma: Optional[torch.Tensor], positions: torch.Tensor,
+                         frequencies: torch.Tensor, *, eps: float = 1e-6, scale: float = 1.0, interleaved: bool = False,
+                         dq: Optional[torch.Tensor] = None, dk: Optional[torch.Tensor] = None):
+    """Gradients ``(dq, dk, dq_gamma, dk_gamma)`` of :func:`norm_rotary` from those of its outputs and its inputs.  The
+    gammas' gradients are float32 sums over all rows in a fixed order (None where there is no gamma).  ``dq`` may be
+    ``dq_out`` or ``q``, ``dk`` likewise."""
+    tensors = (dq_out, dk_out, q, k, q_gamma, k_gamma, positions, frequencies, dq, dk)
+    try:
+        key = ("norm_rotary_backward", interleaved, *map(_layout, tensors))
+        plan = _layouts.get(key)
+    except AttributeError:
+        key = plan = None
+    if plan is None:
+        plan = _remember(key, _rotary_backward_plan(tensors, interleaved))
+    device, dims, strides, code, gamma_code, flags = plan
+    if dq is None:
+        dq = torch.empty_like(q)
+    if dk is None and k is not None:
+        dk = torch.empty_like(k)
     dq_gamma, dk_gamma = (None if g is None else torch.empty_like(g, dtype=torch.float32) for g in (q_gamma, k_gamma))
     _call("asc_cuda_norm_rotary_bwd", device, dq_out.data_ptr(), _ptr(dk_out), q.data_ptr(), _ptr(k), dq.data_ptr(),
           _ptr(dk), _ptr(q_gamma), _ptr(k_gamma), _ptr(dq_gamma), _ptr(dk_gamma), positions.data_ptr(),
-          frequencies.data_ptr(), dims,
-          _PACK[20](*_strides(dq_out), *_strides(dk_out), *_strides(q), *_strides(k), *_strides(dq), *_strides(dk),
-                    *pos_strides), eps, scale, _DTYPE_CODE[q.dtype], gamma_code, 2 | pos_flag | bool(interleaved))
+          frequencies.data_ptr(), dims, strides, eps, scale, code, gamma_code, flags)
     return dq, dk, dq_gamma, dk_gamma
 
 
 # --------------------------------------------------------------------------------------------------
 # Attention to another sequence
 # --------------------------------------------------------------------------------------------------
-def _cross_arguments(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, kv_lengths: Optional[torch.Tensor],
-                     scale: Optional[float]):
+def _cross_arguments(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, kv_lengths: Optional[torch.Tensor]):
+    """Checks what both directions share: device, shapes and the C ABI's dims."""
     device = _device_of("q", q)
     dtype = q.dtype
     if dtype not in (torch.float16, torch.bfloat16):
@@ -275,9 +327,19 @@ def _cross_arguments(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, kv_lengt
         _check_shape("kv_lengths", kv_lengths.shape, (batch, ))
         if not kv_lengths.is_contiguous():
             raise ValueError("kv_lengths must be contiguous")
-    if scale is None:
-        scale = head_dim**-0.5 if head_dim else 0.0
-    return device, q_shape, k_shape, _PACK[6](batch, seq, kv_seq, heads, kv_heads, head_dim), scale
+    return device, q_shape, k_shape, _PACK[6](batch, seq, kv_seq, heads, kv_heads, head_dim)
+
+
+def _default_scale(q: torch.Tensor) -> float:
+    return q.shape[3]**-0.5 if q.shape[3] else 0.0
+
+
+def _cross_plan(tensors):
+    q, k, v, kv_lengths, out = tensors
+    device, q_shape, _, dims = _cross_arguments(q, k, v, kv_lengths)
+    out = _output("out", out, q, q_shape, device)
+    strides = _PACK[12](*_strides(q), *_strides(k), *_strides(v), *_strides(out))
+    return device, dims, strides, _DTYPE_CODE[q.dtype], (q_shape[0], q_shape[2], q_shape[1])
 
 
 def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, kv_lengths: Optional[torch.Tensor] = None,
@@ -289,13 +351,38 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, kv_len
     one state (``expand``) over batch or heads.  S = 1 is the form for generated tokens: few rows are cut along the keys
     and joined.  ``return_lse`` adds the float32 [B, Hq, S] logarithms of the softmax sums, which the gradient needs; a
     query without keys gives 0 and -inf.  Returns ``out`` or ``(out, lse)``."""
-    device, q_shape, _, dims, scale = _cross_arguments(q, k, v, kv_lengths, scale)
-    out = _output("out", out, q, q_shape, device)
-    lse = torch.empty(q_shape[0], q_shape[2], q_shape[1], dtype=torch.float32, device=q.device) if return_lse else None
+    tensors = (q, k, v, kv_lengths, out)
+    try:
+        key = ("cross_attention", *map(_layout, tensors))
+        plan = _layouts.get(key)
+    except AttributeError:
+        key = plan = None
+    if plan is None:
+        plan = _remember(key, _cross_plan(tensors))
+    device, dims, strides, code, lse_shape = plan
+    if out is None:
+        out = torch.empty_like(q)
+    lse = torch.empty(lse_shape, dtype=torch.float32, device=q.device) if return_lse else None
     _call("asc_cuda_cross_attn_fwd_f16", device, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), _ptr(lse),
-          _ptr(kv_lengths), dims, _PACK[12](*_strides(q), *_strides(k), *_strides(v), *_strides(out)), scale,
-          _DTYPE_CODE[q.dtype])
+          _ptr(kv_lengths), dims, strides, _default_scale(q) if scale is None else scale, code)
     return (out, lse) if return_lse else out
+
+
+def _cross_backward_plan(tensors):
+    dout, q, k, v, out, lse, kv_lengths, dq, dk, dv = tensors
+    device, q_shape, k_shape, dims = _cross_arguments(q, k, v, kv_lengths)
+    dtype = q.dtype
+    _check_shape("dout", _check_rows("dout", dout, dtype, device), q_shape)
+    _check_shape("out", _check_rows("out", out, dtype, device), q_shape)
+    _check_vector("lse", lse, (torch.float32, ), device)
+    _check_shape("lse", lse.shape, (q_shape[0], q_shape[2], q_shape[1]))
+    if not lse.is_contiguous():
+        raise ValueError("lse must be contiguous")
+    dq = _output("dq", dq, q, q_shape, device)
+    dk, dv = _output("dk", dk, k, k_shape, device), _output("dv", dv, v, k_shape, device)
+    strides = _PACK[24](*_strides(dout), *_strides(q), *_strides(k), *_strides(v), *_strides(out), *_strides(dq),
+                        *_strides(dk), *_strides(dv))
+    return device, dims, strides, _DTYPE_CODE[dtype]
 
 
 def cross_attention_backward(dout: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out: torch.Tensor,
@@ -306,18 +393,19 @@ def cross_attention_backward(dout: torch.Tensor, q: torch.Tensor, k: torch.Tenso
     (of the same lengths and scale).  Keys that do not take part get 0; where k or v repeat one state over batch or heads,
     dk and dv hold one gradient for each entry.  Every sum is taken in a fixed order.  The outputs must not overlap the
     inputs."""
-    device, q_shape, k_shape, dims, scale = _cross_arguments(q, k, v, kv_lengths, scale)
-    dtype = q.dtype
-    _check_shape("dout", _check_rows("dout", dout, dtype, device), q_shape)
-    _check_shape("out", _check_rows("out", out, dtype, device), q_shape)
-    _check_vector("lse", lse, (torch.float32, ), device)
-    _check_shape("lse", lse.shape, (q_shape[0], q_shape[2], q_shape[1]))
-    if not lse.is_contiguous():
-        raise ValueError("lse must be contiguous")
-    dq = _output("dq", dq, q, q_shape, device)
-    dk, dv = _output("dk", dk, k, k_shape, device), _output("dv", dv, v, k_shape, device)
+    tensors = (dout, q, k, v, out, lse, kv_lengths, dq, dk, dv)
+    try:
+        key = ("cross_attention_backward", *map(_layout, tensors))
+        plan = _layouts.get(key)
+    except AttributeError:
+        key = plan = None
+    if plan is None:
+        plan = _remember(key, _cross_backward_plan(tensors))
+    device, dims, strides, code = plan
+    dq = torch.empty_like(q) if dq is None else dq
+    dk = torch.empty_like(k) if dk is None else dk
+    dv = torch.empty_like(v) if dv is None else dv
     _call("asc_cuda_cross_attn_bwd_f16", device, dout.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(),
-          lse.data_ptr(), _ptr(kv_lengths), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), dims,
-          _PACK[24](*_strides(dout), *_strides(q), *_strides(k), *_strides(v), *_strides(out), *_strides(dq),
-                    *_strides(dk), *_strides(dv)), scale, _DTYPE_CODE[dtype])
+          lse.data_ptr(), _ptr(kv_lengths), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), dims, strides,
+          _default_scale(q) if scale is None else scale, code)
     return dq, dk, dv

@@ -129,8 +129,7 @@ def last_cuda_error() -> str:
 
 def call(fn_name: str, *args) -> None:
     """Call an entry point; non-zero status -> RuntimeError (reference: state.py:64-75)."""
-    fn = getattr(load(), fn_name)
-    error = fn(*args)
+    error = getattr(_lib or load(), fn_name)(*args)
     if error != 0:
         detail = status_string(error)
         if error == 4:
