@@ -2459,7 +2459,9 @@ def _match_matmul_then_program(trace: KernelTrace, eff: Effect) -> Optional[Plan
 
 
 # --------------------------------------------------------------------------------------------------
-# Pattern: attention forward, written per query tile as softmax(scale * Q K^T [+ causal mask]) V
+# Pattern: attention forward, written per query tile as softmax(scale * Q K^T [+ causal mask]) V.  Q, K and V of one shape
+# and head size 128 are self-attention; otherwise (another number of keys, several query heads for one key head, other head
+# sizes) it is attention to another sequence, without a mask.
 # --------------------------------------------------------------------------------------------------
 def _match_attention(trace: KernelTrace, eff: Effect) -> Optional[Plan]:
     value, out_t = eff.args
@@ -2510,18 +2512,28 @@ def _match_attention(trace: KernelTrace, eff: Effect) -> Optional[Plan]:
     rows, D = out_t.static_shape()
     tq = qv.shape[0]
     S = kv.shape[0]
-    if any(t.static_shape() != (rows, D) for t in (qv.tensor, kv.tensor, vv.tensor)):
-        raise _unsupported("attention Q, K, V, O must have the same [rows, head_dim] shape")
-    if qv.shape[1] != D or kv.shape != (S, D) or vv.shape != (S, D) or rows % S != 0 or S % tq != 0:
+    k_rows = kv.tensor.static_shape()[0]
+    if qv.tensor.static_shape() != (rows, D) or any(t.static_shape() != (k_rows, D) for t in (kv.tensor, vv.tensor)):
+        raise _unsupported("attention Q and O, and K and V, must have the same [rows, head_dim] shape")
+    if qv.shape[1] != D or kv.shape != (S, D) or vv.shape != (S, D) or k_rows % S != 0:
         raise _unsupported("attention tiles must span the head dimension, K/V tiles one whole sequence")
+    heads = k_rows // S                                # sequences of keys
+    per = rows // heads if heads else 0                # query rows of each
+    if heads == 0 or rows % heads != 0 or per % tq != 0:
+        raise _unsupported("attention query tiles must divide the query rows of each K/V sequence")
+    cross = not causal and (rows != k_rows or D != 128)
+    if causal and rows != k_rows:
+        raise _unsupported("attention with a causal mask needs as many queries as keys")
+    if cross and (D % 8 != 0 or D > 128):
+        raise _unsupported("attention to another sequence needs a head dimension that is a multiple of 8 up to 128")
     env = enumerate_instances(trace.core_num, eff.loops, eff.guards)
     n = env_count(env)
     row0 = eval_int(eff.attrs["offsets"][0], env, n)
     checks = [
         np.array_equal(np.sort(row0), np.arange(0, rows, tq)),
         np.array_equal(eval_int(qv.offsets[0], env, n), row0),
-        np.array_equal(eval_int(kv.offsets[0], env, n), (row0 // S) * S),
-        np.array_equal(eval_int(vv.offsets[0], env, n), (row0 // S) * S),
+        np.array_equal(eval_int(kv.offsets[0], env, n), (row0 // per) * S),
+        np.array_equal(eval_int(vv.offsets[0], env, n), (row0 // per) * S),
         all(not np.any(eval_int(x.offsets[1], env, n)) for x in (qv, kv, vv)),
         not np.any(eval_int(eff.attrs["offsets"][1], env, n)),
     ]
@@ -2539,9 +2551,26 @@ def _match_attention(trace: KernelTrace, eff: Effect) -> Optional[Plan]:
     plan.writes.add(idx[3])
     if rows * D != out_t.base.numel:
         plan.partial_writes.add(idx[3])
-    heads = rows // S
-
     head_bytes = S * D * 2
+    q_bytes = per * D * 2
+
+    def make_cross(lo: int, hi: int) -> List[Step]:
+        # the query heads that share a sequence of keys are rows of one batch entry
+        dims = (ctypes.c_int64 * 6)(hi - lo, per, S, 1, 1, D)
+        strides = (ctypes.c_int64 * 12)(per * D, D, D, S * D, D, D, S * D, D, D, per * D, D, D)
+
+        def build(ptrs, stream, lo=lo):
+            return (_p(ptrs[idx[0]] + lo * q_bytes), _p(ptrs[idx[1]] + lo * head_bytes), _p(ptrs[idx[2]] + lo * head_bytes),
+                    _p(ptrs[idx[3]] + lo * q_bytes), None, None, dims, strides, ctypes.c_float(scale),
+                    ctypes.c_int32(_DTYPE_CODE_16[dt.name]), stream)
+        return [Step("asc_cuda_cross_attn_fwd_f16", build, f"{hi - lo} sequences x {per} queries x {S} keys x {D}")]
+
+    if cross:
+        plan.steps += make_cross(0, heads)
+        if not plan.partial_writes and len(set(idx)) == 4:
+            streamed = {idx[0]: q_bytes, idx[1]: head_bytes, idx[2]: head_bytes, idx[3]: q_bytes}
+            plan.pipeline = PipelineSpec(heads, 1, streamed, set(), make_cross)
+        return plan
 
     def make(lo: int, hi: int) -> List[Step]:
         def build(ptrs, stream, lo=lo, hi=hi):
