@@ -350,8 +350,9 @@ int32_t asc_cuda_norm_rotary_bwd(const void* dq_out, const void* dk_out, const v
  * strides, in elements, the last dimension contiguous: q, k, v, o (three each: batch, sequence, head).  All four 16-byte
  * aligned with strides in multiples of 8 elements; the batch and head strides of k and v may be 0 (one state for several
  * entries).  dims and strides are host arrays.  scale >= 0.  dtype: 0 fp16, 1 bf16; fp32 softmax and accumulation, the
- * probabilities rounded to dtype for the second product.  o must not overlap k or v.  Few rows are cut along the keys
- * and joined in a fixed order; that workspace is allocated and released on the stream.  No counterpart in the reference. */
+ * probabilities rounded to dtype for the second product.  o may be q (same pointer and strides) and must not overlap k or
+ * v.  Where rows are few or do not fill the SMs they are cut along the keys and joined in a fixed order; a workspace for
+ * that is allocated and released on the stream.  No counterpart in the reference. */
 int32_t asc_cuda_cross_attn_fwd_f16(const void* q, const void* k, const void* v, void* o, float* lse,
                                     const int32_t* kv_lengths, const int64_t* dims, const int64_t* strides, float scale,
                                     int32_t dtype, void* stream);

@@ -4,7 +4,9 @@ keys, alone or behind an RMS norm of every head, and attention to the states of 
 The functions are thin: they check their arguments (``ValueError`` / ``TypeError``), allocate outputs with torch, and
 make one call of the C ABI (``include/asc_cuda.h``) on torch's current stream of the tensors' device.  They return
 without waiting for the GPU and record no autograd history; every operator's gradient is a function of its own.  A
-status other than 0 raises ``RuntimeError`` (:func:`pyasc_b200.capi.call`).
+status other than 0 raises ``RuntimeError`` (:func:`pyasc_b200.capi.call`); a device-side wait that ran out shows at the
+next :func:`pyasc_b200.capi.check_device_status`.  Calls may be captured into CUDA graphs, the first ones too; workspaces
+belong to a call, so calls and graphs may run at the same time on several streams.
 
 Tensors are [batch, sequence, heads, head_dim] with any strides, as long as the last dimension is contiguous: slices of
 a packed projection, or ``x.transpose(1, 2)`` of a [batch, heads, sequence, head_dim] tensor.
@@ -350,7 +352,8 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, kv_len
     keys from there on do not take part, whatever they hold.  ``scale`` is ``D ** -0.5`` unless given.  k and v may repeat
     one state (``expand``) over batch or heads.  S = 1 is the form for generated tokens: few rows are cut along the keys
     and joined.  ``return_lse`` adds the float32 [B, Hq, S] logarithms of the softmax sums, which the gradient needs; a
-    query without keys gives 0 and -inf.  Returns ``out`` or ``(out, lse)``."""
+    query without keys gives 0 and -inf.  ``out`` may be ``q`` and must not overlap k or v.  Returns ``out`` or
+    ``(out, lse)``."""
     tensors = (q, k, v, kv_lengths, out)
     try:
         key = ("cross_attention", *map(_layout, tensors))

@@ -933,6 +933,7 @@ int32_t launch_fwd(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorM
   int dev = 0;
   ASC_CUDA_TRY(cudaGetDevice(&dev));
   if (!attr_set.get(dev)) {
+    aschost::SetUpInCapture relaxed;
     // refuse to launch a build whose register split would wait forever (see attention.cu)
     cudaFuncAttributes fa{};
     ASC_CUDA_TRY(cudaFuncGetAttributes(&fa, kernel));

@@ -599,6 +599,7 @@ int32_t launch_bwd(const Maps& k_maps, const Maps& q_maps, const BwdParams& pk, 
   int dev = 0;
   ASC_CUDA_TRY(cudaGetDevice(&dev));
   if (!attr_set.get(dev)) {
+    aschost::SetUpInCapture relaxed;
     // refuse to launch a build whose register split would wait forever (see attention.cu)
     cudaFuncAttributes fa{};
     ASC_CUDA_TRY(cudaFuncGetAttributes(&fa, kernel));

@@ -42,6 +42,20 @@ int32_t encode_tmap(CUtensorMap* out, CUtensorMapDataType dtype, uint32_t rank, 
 int32_t scratch_alloc(void** out, size_t bytes, cudaStream_t stream);
 int32_t scratch_free(void* ptr, cudaStream_t stream);
 
+// While one of these lives, this thread may make set-up calls that a stream capture in progress would otherwise refuse
+// (and be invalidated by): creating a pool, looking up an address, loading a kernel to set its attributes.  None of them
+// touches the captured stream, so a first call may come inside a capture.
+class SetUpInCapture {
+ public:
+  SetUpInCapture() { cudaThreadExchangeStreamCaptureMode(&mode_); }
+  ~SetUpInCapture() { cudaThreadExchangeStreamCaptureMode(&mode_); }
+  SetUpInCapture(const SetUpInCapture&) = delete;
+  SetUpInCapture& operator=(const SetUpInCapture&) = delete;
+
+ private:
+  cudaStreamCaptureMode mode_ = cudaStreamCaptureModeRelaxed;
+};
+
 // Kernels launched by this library since load.
 extern std::atomic<uint64_t> g_launch_count;
 inline void count_launch() { g_launch_count.fetch_add(1, std::memory_order_relaxed); }

@@ -44,6 +44,7 @@ int32_t device_status_word(uint32_t** out) {
   if (dev < 0 || dev >= kMaxDevices) return ASC_ERR_INVALID_ARG;
   std::lock_guard<std::mutex> lock(g_mutex);
   if (g_status_ptr[dev] == nullptr) {
+    SetUpInCapture relaxed;
     void* p = nullptr;
     ASC_CUDA_TRY(cudaGetSymbolAddress(&p, g_device_status));
     g_status_ptr[dev] = static_cast<uint32_t*>(p);
@@ -77,6 +78,7 @@ int32_t scratch_alloc(void** out, size_t bytes, cudaStream_t stream) {
   {
     std::lock_guard<std::mutex> lock(g_mutex);
     if (g_scratch_pool[dev] == nullptr) {
+      SetUpInCapture relaxed;
       cudaMemPoolProps props = {};
       props.allocType = cudaMemAllocationTypePinned;
       props.handleTypes = cudaMemHandleTypeNone;

@@ -58,3 +58,39 @@ def test_host_tensors_are_refused():
         A.cross_attention(q, q, q)
     with pytest.raises(TypeError):
         A.cross_attention(None, q, q)
+
+
+def test_a_call_runs_on_its_tensors_device(monkeypatch):
+    """With another device current, the tensors' device is made current for the call, and its stream is used."""
+    seen = []
+
+    class Current:
+        device = 0
+
+        def __init__(self, device):
+            self.to = device
+
+        def __enter__(self):
+            self.back, Current.device = Current.device, self.to
+
+        def __exit__(self, *_):
+            Current.device = self.back
+
+    monkeypatch.setattr(torch._C, "_cuda_getDevice", lambda: Current.device, raising=False)
+    monkeypatch.setattr(torch._C, "_cuda_getCurrentRawStream", lambda device: 100 + device, raising=False)
+    monkeypatch.setattr(torch.cuda, "device", Current)
+    monkeypatch.setattr(capi, "call", lambda name, *args: seen.append((Current.device, name, args)))
+    A._call("f", 1, 7)
+    A._call("g", 0, 8)
+    assert seen == [(1, "f", (7, 101)), (0, "g", (8, 100))] and Current.device == 0
+
+
+def test_layouts_that_are_kept_are_bounded():
+    before = dict(A._layouts)
+    try:
+        for i in range(A._MAX_LAYOUTS + 10):
+            A._remember(("test", i), (i, ))
+        assert len(A._layouts) <= A._MAX_LAYOUTS
+    finally:
+        A._layouts.clear()
+        A._layouts.update(before)

@@ -63,6 +63,8 @@ SIZES = [
     (1, 700, 1025, 4, 2, 128),
     (2, 513, 640, 4, 4, 64),
     (1, 300, 1, 2, 2, 8),
+    (1, 1, 700, 64, 1, 128),
+    (2, 3, 130, 17, 1, 64),
     (60, 256, 200, 4, 4, 64),
     (40, 3, 513, 8, 8, 128),
 ]

@@ -52,6 +52,8 @@ SIZES = [
     (1, 40, 5000, 2, 1, 128),
     (1, 5000, 40, 2, 1, 128),
     (1, 300, 1, 2, 2, 8),
+    (1, 1, 700, 64, 1, 128),
+    (2, 3, 130, 17, 1, 64),
     (40, 130, 260, 4, 4, 128),
 ]
 

@@ -1,5 +1,9 @@
 """The attention part of an encoder-decoder block as it is used: per-head norms and rotary positions of packed queries and
 keys, causal self-attention, attention to padded encoder states, and back through both; in prompts and token by token."""
+import os
+import subprocess
+import sys
+
 import pytest
 import torch
 
@@ -112,3 +116,32 @@ def test_calls_on_two_streams_at_once():
     torch.cuda.synchronize()
     for x in got:
         assert all(torch.equal(a, b) for a, b in zip(x, (*want, *grads)))
+
+
+FIRST_CALLS_IN_A_CAPTURE = """
+import torch
+from pyasc_b200 import attention as A
+q, k, p = (torch.randn(2, n, h, 64, device="cuda").half() for n, h in ((1, 4), (3000, 2), (300, 4)))
+frequencies, _ = A.rotary_frequencies(64, device="cuda")
+positions, gamma = torch.arange(300, device="cuda"), torch.ones(64, device="cuda")
+
+def step():
+    x, _ = A.norm_rotary(p, None, gamma, None, positions, frequencies)
+    y, lse = A.cross_attention(x, k, k, return_lse=True)
+    return (x, y, *A.cross_attention_backward(p, x, k, k, y, lse), A.cross_attention(q, k, k),
+            A.norm_rotary_backward(p, None, p, None, gamma, None, positions, frequencies)[2])
+
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    got = step()
+graph.replay()
+torch.cuda.synchronize()
+assert all(torch.equal(a, b) for a, b in zip(got, step()))
+"""
+
+
+def test_first_calls_inside_a_capture():
+    """A process whose first calls are captured: what the library sets up on first use does not break the capture."""
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    done = subprocess.run([sys.executable, "-c", FIRST_CALLS_IN_A_CAPTURE], cwd=root, capture_output=True, text=True, timeout=300)
+    assert done.returncode == 0, done.stderr[-2000:]
