@@ -678,8 +678,9 @@ int32_t run(const Call& c) {
              static_cast<int32_t>(c.B * c.Hkv * kv_tiles), 0, 0};
   pq.work = {c.lengths, p.B, p.Skv, p.Hkv, static_cast<int32_t>(q_tiles), 0, kStep,
              static_cast<int32_t>(c.B * c.Hkv * q_tiles), 0, 0};
-  // The passes share the SMs: each item an SM of its own where that is enough, otherwise by their products (a step has
-  // four for keys, three for queries, and what a step costs besides).
+  // The passes share the SMs: each item an SM of its own where that is enough, otherwise by what a step costs, four
+  // products for keys against three for queries and the same chain of waits: 6 to 5 (measured at [2, 2048] on 4096, 32 / 8
+  // heads of 128: 822 us; 6 to 4.7: 861, 6 to 5.3: 838).
   const int64_t q_steps = (c.Skv + kStep - 1) / kStep;
   int k_sms = 0;
   if (c.Skv > 0) {
