@@ -74,6 +74,11 @@ __device__ __forceinline__ bool elect_one() {
   return one != 0;
 }
 
+// Two kernels of one call, the second launched with aschost::launch_after: the first lets the second's CTAs start where it
+// leaves room, and the second waits for all of the first's results before it reads or writes anything they share.
+__device__ __forceinline__ void let_next_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void wait_for_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
 // ------------------------------- mbarrier ---------------------------------
 __device__ __forceinline__ void mbar_init(uint32_t bar, uint32_t count) {
   asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count) : "memory");

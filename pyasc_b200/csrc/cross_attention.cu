@@ -297,6 +297,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     tmem_alloc(smem_u32(&ctl.tmem_base), 512);
     tmem_relinquish();
   }
+  let_next_start();
   if (warp == 10) ascsched::find_range(p.work, blockIdx.x, gridDim.x, &range);
   tc_fence_before();
   __syncthreads();
@@ -591,6 +592,7 @@ __global__ void __launch_bounds__(kFewWarps * 32, 2) cross_few_kernel(const Cros
   __shared__ Range range;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
   if (!kCluster) {
+    let_next_start();
     if (warp == 0) ascsched::find_range(p.work, blockIdx.x, gridDim.x, &range);
     __syncthreads();
   }
@@ -831,6 +833,7 @@ __global__ void __launch_bounds__(256) cross_join_kernel(const CrossParams p, in
     const bool is = ascsched::find_cut(p.work, blockIdx.x + 1, ctas, mine);
     if (threadIdx.x == 0) cut = mine, found = is;
   }
+  wait_for_previous();
   __syncthreads();
   if (!found) return;
   const int per_row = p.D / 4, abreast = 256 / per_row;          // rows the CTA works on side by side
@@ -891,9 +894,9 @@ __global__ void __launch_bounds__(256) cross_join_kernel(const CrossParams p, in
 template <bool kBf16, int kTiles>
 int32_t launch_join(const CrossParams& p, int ctas, cudaStream_t stream) {
   const int rows = kTiles == 0 ? kFewRows : kTiles * kTileQ, per_cta = 256 / (p.D / 4) * kJoinRows;
-  cross_join_kernel<kBf16, kTiles><<<dim3(ctas - 1, (rows + per_cta - 1) / per_cta), 256, 0, stream>>>(p, ctas);
+  ASC_CUDA_TRY(aschost::launch_after(cross_join_kernel<kBf16, kTiles>, dim3(ctas - 1, (rows + per_cta - 1) / per_cta), dim3(256),
+                                     0, stream, p, ctas));
   aschost::count_launch();
-  ASC_CUDA_TRY(cudaGetLastError());
   return ASC_OK;
 }
 

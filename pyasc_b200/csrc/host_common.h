@@ -56,6 +56,23 @@ class SetUpInCapture {
   cudaStreamCaptureMode mode_ = cudaStreamCaptureModeRelaxed;
 };
 
+// Launch of the second of two kernels of one call: it may start before the first has ended and calls
+// ascdev::wait_for_previous() itself.
+template <typename... Params, typename... Args>
+cudaError_t launch_after(void (*kernel)(Params...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream, Args... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = block;
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, static_cast<Params>(args)...);
+}
+
 // Kernels launched by this library since load.
 extern std::atomic<uint64_t> g_launch_count;
 inline void count_launch() { g_launch_count.fetch_add(1, std::memory_order_relaxed); }

@@ -373,6 +373,7 @@ template <typename T, bool kInter>
 __global__ void __launch_bounds__(kThreads, 2) rotary_bwd_kernel(const __grid_constant__ RotaryArgs a) {
   constexpr int E = Vec<T>::E;
   extern __shared__ float smem[];
+  ascdev::let_next_start();
   float2* table = stage(a, smem);
   // [queries, keys][pair][thread], behind the angles
   float2* sums = reinterpret_cast<float2*>(smem + 2 * a.D) + kWarps * (a.r / 2);
@@ -630,6 +631,7 @@ __global__ void __launch_bounds__(32 * kSumParts) dgamma_kernel(const float* par
   const int lo = blockIdx.y ? q_rows : 0, hi = blockIdx.y ? rows : q_rows;
   float* out = blockIdx.y ? dk_gamma : dq_gamma;
   double t = 0.0;
+  ascdev::wait_for_previous();
   if (c < D)
     for (int i = lo + part; i < hi; i += 8 * kSumParts) {
       float x[8];
@@ -823,9 +825,8 @@ int32_t launch_bwd(RotaryArgs a, const Problem& pr, float* dq_gamma, float* dk_g
   if (e == cudaSuccess) {
     aschost::count_launch();
     if (ws != nullptr) {
-      dgamma_kernel<<<dim3((a.D + 31) / 32, 2), 32 * kSumParts, 0, st>>>(a.partial, a.q_ctas, static_cast<int>(n_rows), a.D, dq_gamma,
-                                                              dk_gamma);
-      e = cudaGetLastError();
+      e = aschost::launch_after(dgamma_kernel, dim3((a.D + 31) / 32, 2), dim3(32 * kSumParts), 0, st, a.partial, a.q_ctas,
+                                static_cast<int>(n_rows), a.D, dq_gamma, dk_gamma);
       if (e == cudaSuccess) aschost::count_launch();
     }
   }
