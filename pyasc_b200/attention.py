@@ -201,7 +201,7 @@ def _gammas(device: int, head_dim: int, q_gamma: Optional[torch.Tensor], k_gamma
 
 
 def _rotary_plan(tensors, interleaved, flags):
-    """Checks of a forward call: device, codes of the types, flags, dims, and strides but for those of the outputs."""
+    """Checks of a forward call: device, dims, strides, codes of the types, flags."""
     q, k, q_gamma, k_gamma, positions, frequencies, q_out, k_out = tensors
     device, q_shape, k_shape, dims, pos_strides, pos_flag = _rotary_arguments(q, k, positions, frequencies)
     if k is None and (k_out is not None or k_gamma is not None):

@@ -310,3 +310,40 @@ def test_in_place_backward():
     got = A.norm_rotary_backward(a, dk, q, b, g, g, pos, freq, dq=a, dk=b)
     assert got[0] is a and got[1] is b
     assert all(torch.equal(x, y) for x, y in zip(got, want))
+
+
+def test_refusals():
+    q, k = normal((2, 4, 4, 64), torch.float16, 1), normal((2, 4, 2, 64), torch.float16, 2)
+    pos, g = torch.arange(4, device="cuda"), torch.ones(64, device="cuda")
+    freq, _ = A.rotary_frequencies(64, device="cuda")
+    wide, _ = A.rotary_frequencies(66, device="cuda")
+    calls = [
+        (ValueError, lambda: A.rotary(q, k[:1], pos, freq)),
+        (ValueError, lambda: A.rotary(q, k[:, :3], pos, freq)),
+        (ValueError, lambda: A.rotary(q, k[..., :32], pos, freq)),
+        (ValueError, lambda: A.rotary(q[0], None, pos, freq)),
+        (ValueError, lambda: A.rotary(q.transpose(2, 3), None, pos, freq)),
+        (ValueError, lambda: A.rotary(q, k.cpu(), pos, freq)),
+        (TypeError, lambda: A.rotary(q, k.float(), pos, freq)),
+        (TypeError, lambda: A.rotary(q.double(), None, pos, freq)),
+        (TypeError, lambda: A.rotary(q, k, pos.float(), freq)),
+        (ValueError, lambda: A.rotary(q, k, pos[:3], freq)),
+        (ValueError, lambda: A.rotary(q, k, pos.expand(3, 4), freq)),
+        (TypeError, lambda: A.rotary(q, k, pos, freq.float())),
+        (ValueError, lambda: A.rotary(q, k, pos, wide)),
+        (ValueError, lambda: A.rotary(q, k, pos, freq.expand(2, -1))),
+        (ValueError, lambda: A.rotary(q, k, pos, freq, q_out=torch.empty_like(k))),
+        (ValueError, lambda: A.rotary(q, k, pos, freq, q_out=q[:1].expand(2, -1, -1, -1))),
+        (ValueError, lambda: A.rotary(q, None, pos, freq, k_out=k)),
+        (ValueError, lambda: A.norm_rotary(q, k, g[:32], g, pos, freq)),
+        (TypeError, lambda: A.norm_rotary(q, k, g, g.half(), pos, freq)),
+        (ValueError, lambda: A.norm_rotary(q, None, g, g, pos, freq)),
+        (ValueError, lambda: A.norm_rotary_backward(q, None, q, k, g, g, pos, freq)),
+        (ValueError, lambda: A.norm_rotary_backward(q[:, :3], k, q, k, g, g, pos, freq)),
+        (ValueError, lambda: A.norm_rotary_backward(q, k, q, k, g, g, pos, freq, dk=q)),
+        (RuntimeError, lambda: A.rotary(q.repeat(1, 1, 1, 17), None, pos, freq)),       # a head of 1088
+    ]
+    A.rotary(q, k, pos, freq)                      # (an allowed call does not let a refused one through)
+    for error, call in calls:
+        with pytest.raises(error):
+            call()
