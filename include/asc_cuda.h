@@ -326,8 +326,8 @@ int32_t asc_cuda_attn_fwd_f16(const void* q, const void* k, const void* v, void*
  * positions (batch, sequence; 0 repeats); an output stride of 0 over several elements is status 1.  dims and strides
  * are host arrays.  dtype: 0 fp16, 1 bf16, 2 fp32 of q, k and the outputs; gamma_dtype the same for the gammas.  fp32
  * arithmetic, one rounding at the store.  An output may be its input (same pointer and strides).  Pointers need their
- * element's alignment; operands whose pointers and strides are multiples of 16 bytes, with D (and r / 2 for halves) a
- * multiple of 16 bytes too, take the vector kernels.  No counterpart in the reference. */
+ * element's alignment; operands whose pointers and strides are multiples of 16 bytes (8 for fp16 and bf16), with D (and
+ * r / 2 for halves) multiples of them too, take the vector kernels.  No counterpart in the reference. */
 int32_t asc_cuda_norm_rotary(const void* q, const void* k, void* q_out, void* k_out, const void* q_gamma,
                              const void* k_gamma, const void* positions, const double* frequencies,
                              const int64_t* dims, const int64_t* strides, float eps, float scale, int32_t dtype,

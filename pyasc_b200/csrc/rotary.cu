@@ -62,57 +62,62 @@ __device__ __forceinline__ __half from_float<__half>(float v) { return __float2h
 template <>
 __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 
-// 16 bytes of a row <-> fp32 registers
-template <typename T>
-struct Vec;
+// kBytes (16 or 8) of a row <-> fp32 registers
+template <int kBytes>
+struct RawOf;
 template <>
-struct Vec<float> {
+struct RawOf<16> {
+  using Type = uint4;
+  __device__ static uint4 zero() { return make_uint4(0, 0, 0, 0); }
+};
+template <>
+struct RawOf<8> {
+  using Type = uint2;
+  __device__ static uint2 zero() { return make_uint2(0, 0); }
+};
+__device__ __forceinline__ float2 unpack2(uint32_t w, const __half*) { return __half22float2(*reinterpret_cast<const __half2*>(&w)); }
+__device__ __forceinline__ float2 unpack2(uint32_t w, const __nv_bfloat16*) {
+  return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+}
+__device__ __forceinline__ uint32_t pack2(float a, float b, const __half*) {
+  const __half2 h = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ uint32_t pack2(float a, float b, const __nv_bfloat16*) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+template <typename T, int kBytes>
+struct Vec {
+  static constexpr int E = kBytes / 2;
+  using Raw = typename RawOf<kBytes>::Type;
+  __device__ static Raw zero() { return RawOf<kBytes>::zero(); }
+  __device__ static void unpack(const Raw& t, float* v) {
+    const uint32_t* w = reinterpret_cast<const uint32_t*>(&t);
+#pragma unroll
+    for (int i = 0; i < E / 2; ++i) {
+      const float2 f = unpack2(w[i], static_cast<const T*>(nullptr));
+      v[2 * i] = f.x, v[2 * i + 1] = f.y;
+    }
+  }
+  __device__ static Raw pack(const float* v) {
+    Raw t;
+    uint32_t* w = reinterpret_cast<uint32_t*>(&t);
+#pragma unroll
+    for (int i = 0; i < E / 2; ++i) w[i] = pack2(v[2 * i], v[2 * i + 1], static_cast<const T*>(nullptr));
+    return t;
+  }
+};
+template <>
+struct Vec<float, 16> {
   static constexpr int E = 4;
+  using Raw = uint4;
+  __device__ static uint4 zero() { return make_uint4(0, 0, 0, 0); }
   __device__ static void unpack(const uint4& t, float* v) {
     v[0] = __uint_as_float(t.x), v[1] = __uint_as_float(t.y), v[2] = __uint_as_float(t.z), v[3] = __uint_as_float(t.w);
   }
   __device__ static uint4 pack(const float* v) {
     return make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
-  }
-};
-template <>
-struct Vec<__half> {
-  static constexpr int E = 8;
-  __device__ static void unpack(const uint4& t, float* v) {
-    const uint32_t w[4] = {t.x, t.y, t.z, t.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
-      v[2 * i] = f.x, v[2 * i + 1] = f.y;
-    }
-  }
-  __device__ static uint4 pack(const float* v) {
-    uint32_t w[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const __half2 h = __floats2half2_rn(v[2 * i], v[2 * i + 1]);
-      w[i] = *reinterpret_cast<const uint32_t*>(&h);
-    }
-    return make_uint4(w[0], w[1], w[2], w[3]);
-  }
-};
-template <>
-struct Vec<__nv_bfloat16> {
-  static constexpr int E = 8;
-  __device__ static void unpack(const uint4& t, float* v) {
-    const uint32_t w[4] = {t.x, t.y, t.z, t.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      v[2 * i] = __uint_as_float(w[i] << 16), v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
-  }
-  __device__ static uint4 pack(const float* v) {
-    uint32_t w[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const __nv_bfloat162 h = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
-      w[i] = *reinterpret_cast<const uint32_t*>(&h);
-    }
-    return make_uint4(w[0], w[1], w[2], w[3]);
   }
 };
 
@@ -143,7 +148,7 @@ __device__ __forceinline__ T* row_of(const Operand& o, int b, int s, int h) {
   return static_cast<T*>(o.p) + b * o.b + s * o.s + h * o.h;
 }
 
-// Which two 16-byte vectors of a row a lane owns.  Half layout: lane < r / 2 / E owns the vectors of both halves of its
+// Which two vectors (of 16 or 8 bytes, E elements) of a row a lane owns.  Half layout: lane < r / 2 / E owns the vectors of both halves of its
 // pairs; later lanes own two neighbours of the part that is not turned.  Interleaved: both halves of a pair lie in one
 // vector, and a lane owns vectors `lane` and `lane + ceil(n / 2)`.
 template <int E>
@@ -265,25 +270,29 @@ struct Place {
 };
 
 // The vectors of one tensor's rows that a lane owns, as a pointer that walks over the heads of a token.
-template <typename T>
+template <typename T, int kBytes>
 struct RowWalk {
-  const uint4* at;
-  int64_t stride;            // in 16-byte vectors
+  using V = Vec<T, kBytes>;
+  using Raw = typename V::Raw;
+  const Raw* at;
+  int64_t stride;            // in vectors
   __device__ RowWalk(const Operand& o, const Place& p, int v0, int step)
-      : at(reinterpret_cast<const uint4*>(row_of<const T>(o, p.b, p.s, p.first)) + v0), stride(o.h * step / Vec<T>::E) {}
+      : at(reinterpret_cast<const Raw*>(row_of<const T>(o, p.b, p.s, p.first)) + v0), stride(o.h * step / V::E) {}
   __device__ void next() { at += stride; }
-  __device__ uint4* out() const { return const_cast<uint4*>(at); }
+  __device__ Raw* out() const { return const_cast<Raw*>(at); }
 };
 
 // --------------------------------------------------------------------------------------------------------------
-// Forward, whole 16-byte vectors.  A warp works on one token, or on a slice of its heads where tokens are few: it
+// Forward, whole vectors.  A warp works on one token, or on a slice of its heads where tokens are few: it
 // computes the token's angles into its own piece of shared memory (no barrier beyond the warp), then its groups of
 // lanes take the queries in turn and then the keys.  The next row, also the next token's first, is loaded before the
 // current one is computed.  Warps stride over the tokens.
 // --------------------------------------------------------------------------------------------------------------
-template <typename T, bool kNorm, bool kInter>
+template <typename T, int kBytes, bool kNorm, bool kInter>
 __global__ void __launch_bounds__(kThreads, kFwdCtas) rotary_fwd_kernel(const __grid_constant__ RotaryArgs a) {
-  constexpr int E = Vec<T>::E;
+  using V = Vec<T, kBytes>;
+  using Raw = typename V::Raw;
+  constexpr int E = V::E;
   extern __shared__ float smem[];
   float2* table = stage(a, smem);
   const int lane = threadIdx.x & ((1 << a.log_lanes) - 1), group = (threadIdx.x & 31) >> a.log_lanes;
@@ -300,16 +309,16 @@ __global__ void __launch_bounds__(kThreads, kFwdCtas) rotary_fwd_kernel(const __
     const int b = token / a.S;
     return Place{b, token - b * a.S, (unit - token * a.slices) * groups + group};
   };
-  auto load = [&](const uint4* at, bool on, uint4& lo, uint4& hi) {
-    lo = hi = make_uint4(0, 0, 0, 0);
+  auto load = [&](const Raw* at, bool on, Raw& lo, Raw& hi) {
+    lo = hi = V::zero();
     if (on && l.has0) lo = at[0];
     if (on && l.has1) hi = at[l.v1 - l.v0];
   };
   int unit = blockIdx.x * kWarps + (threadIdx.x >> 5);
   if (unit >= units) return;
   Place p = place(unit);
-  uint4 lo, hi;
-  load(RowWalk<T>(a.x[w_first], p, l.v0, step).at, p.first < a.heads[w_first], lo, hi);
+  Raw lo, hi;
+  load(RowWalk<T, kBytes>(a.x[w_first], p, l.v0, step).at, p.first < a.heads[w_first], lo, hi);
   double pos = a.r > 0 ? position_at(a, p.b, p.s) : 0.0;
   for (; unit < units; unit += warps) {
     __syncwarp();                                  // the previous token's angles are no longer read
@@ -329,19 +338,19 @@ __global__ void __launch_bounds__(kThreads, kFwdCtas) rotary_fwd_kernel(const __
       if (H == 0) continue;
       const int iters = (H + step - 1) / step;
       if (kNorm) lane_turn<E, kInter, kNorm>(a, l, table, smem + w * a.D, t);
-      RowWalk<T> in(a.x[w], p, l.v0, step), out(a.y[w], p, l.v0, step);
+      RowWalk<T, kBytes> in(a.x[w], p, l.v0, step), out(a.y[w], p, l.v0, step);
       int h = p.first;
       for (int it = 0; it < iters; ++it, h += step) {
         float2 v[E];
-        Vec<T>::unpack(lo, reinterpret_cast<float*>(v));
-        Vec<T>::unpack(hi, reinterpret_cast<float*>(v + E / 2));
+        V::unpack(lo, reinterpret_cast<float*>(v));
+        V::unpack(hi, reinterpret_cast<float*>(v + E / 2));
         if (it + 1 < iters) {
           in.next();
           load(in.at, h + step < H, lo, hi);
         } else if (w == 0 && a.heads[1] > 0) {
-          load(RowWalk<T>(a.x[1], p, l.v0, step).at, p.first < a.heads[1], lo, hi);
+          load(RowWalk<T, kBytes>(a.x[1], p, l.v0, step).at, p.first < a.heads[1], lo, hi);
         } else if (more) {
-          load(RowWalk<T>(a.x[w_first], next, l.v0, step).at, next.first < a.heads[w_first], lo, hi);
+          load(RowWalk<T, kBytes>(a.x[w_first], next, l.v0, step).at, next.first < a.heads[w_first], lo, hi);
         }
         if (kNorm) {
           float2 ss = make_float2(0.f, 0.f);
@@ -353,9 +362,9 @@ __global__ void __launch_bounds__(kThreads, kFwdCtas) rotary_fwd_kernel(const __
         }
         if (h < H) {
           apply<E, kInter>(a, l, t, v);
-          uint4* row = out.out();
-          if (l.has0) row[0] = Vec<T>::pack(reinterpret_cast<float*>(v));
-          if (l.has1) row[l.v1 - l.v0] = Vec<T>::pack(reinterpret_cast<float*>(v + E / 2));
+          Raw* row = out.out();
+          if (l.has0) row[0] = V::pack(reinterpret_cast<float*>(v));
+          if (l.has1) row[l.v1 - l.v0] = V::pack(reinterpret_cast<float*>(v + E / 2));
         }
         out.next();
       }
@@ -365,13 +374,15 @@ __global__ void __launch_bounds__(kThreads, kFwdCtas) rotary_fwd_kernel(const __
 }
 
 // --------------------------------------------------------------------------------------------------------------
-// Backward through norm and rotation, whole 16-byte vectors: the forward's division of the work.  A lane's sums for
+// Backward through norm and rotation, whole vectors: the forward's division of the work.  A lane's sums for
 // dgamma stay in registers over a token's queries (then its keys) and are added to the lane's own place in shared memory
 // after them, so that queries and keys share the angles without two sets of sums in registers.
 // --------------------------------------------------------------------------------------------------------------
-template <typename T, bool kInter>
+template <typename T, int kBytes, bool kInter>
 __global__ void __launch_bounds__(kThreads, 2) rotary_bwd_kernel(const __grid_constant__ RotaryArgs a) {
-  constexpr int E = Vec<T>::E;
+  using V = Vec<T, kBytes>;
+  using Raw = typename V::Raw;
+  constexpr int E = V::E;
   extern __shared__ float smem[];
   ascdev::let_next_start();
   float2* table = stage(a, smem);
@@ -394,13 +405,13 @@ __global__ void __launch_bounds__(kThreads, 2) rotary_bwd_kernel(const __grid_co
     const int b = token / a.S;
     return Place{b, token - b * a.S, (unit - token * a.slices) * groups + group};
   };
-  auto load = [&](const Place& p, int h, uint4 (&x)[2], uint4 (&y)[2]) {
-    x[0] = x[1] = y[0] = y[1] = make_uint4(0, 0, 0, 0);
+  auto load = [&](const Place& p, int h, Raw (&x)[2], Raw (&y)[2]) {
+    x[0] = x[1] = y[0] = y[1] = V::zero();
     if (h >= H) return;
     const int w = h >= a.heads[0];
     const int hw = h - (w ? a.heads[0] : 0);
-    const uint4* xr = reinterpret_cast<const uint4*>(row_of<const T>(a.x[w], p.b, p.s, hw));
-    const uint4* yr = reinterpret_cast<const uint4*>(row_of<const T>(a.dy[w], p.b, p.s, hw));
+    const Raw* xr = reinterpret_cast<const Raw*>(row_of<const T>(a.x[w], p.b, p.s, hw));
+    const Raw* yr = reinterpret_cast<const Raw*>(row_of<const T>(a.dy[w], p.b, p.s, hw));
     if (l.has0) x[0] = xr[l.v0], y[0] = yr[l.v0];
     if (l.has1) x[1] = xr[l.v1], y[1] = yr[l.v1];
   };
@@ -414,7 +425,7 @@ __global__ void __launch_bounds__(kThreads, 2) rotary_bwd_kernel(const __grid_co
   int unit = blockIdx.x * kWarps + (threadIdx.x >> 5);
   if (unit < units) {
     Place p = place(unit);
-    uint4 x[2], y[2];
+    Raw x[2], y[2];
     load(p, p.first, x, y);
     double pos = a.r > 0 ? position_at(a, p.b, p.s) : 0.0;
     for (; unit < units; unit += warps) {
@@ -449,10 +460,10 @@ __global__ void __launch_bounds__(kThreads, 2) rotary_bwd_kernel(const __grid_co
           }
         }
         float2 v[E], d[E];
-        Vec<T>::unpack(x[0], reinterpret_cast<float*>(v));
-        Vec<T>::unpack(x[1], reinterpret_cast<float*>(v + E / 2));
-        Vec<T>::unpack(y[0], reinterpret_cast<float*>(d));
-        Vec<T>::unpack(y[1], reinterpret_cast<float*>(d + E / 2));
+        V::unpack(x[0], reinterpret_cast<float*>(v));
+        V::unpack(x[1], reinterpret_cast<float*>(v + E / 2));
+        V::unpack(y[0], reinterpret_cast<float*>(d));
+        V::unpack(y[1], reinterpret_cast<float*>(d + E / 2));
         if (it + 1 < iters) load(p, h + step, x, y);
         else if (more) load(next, next.first, x, y);
         // d = R^T dy
@@ -489,9 +500,9 @@ __global__ void __launch_bounds__(kThreads, 2) rotary_bwd_kernel(const __grid_co
             dg[e] = __ffma2_rn(v[e], rd, dg[e]);
             d[e] = __ffma2_rn(v[e], k2, __fmul2_rn(g[e], rd));
           }
-          uint4* row = reinterpret_cast<uint4*>(row_of<T>(a.y[w], p.b, p.s, h - (w ? a.heads[0] : 0)));
-          if (l.has0) row[l.v0] = Vec<T>::pack(reinterpret_cast<float*>(d));
-          if (l.has1) row[l.v1] = Vec<T>::pack(reinterpret_cast<float*>(d + E / 2));
+          Raw* row = reinterpret_cast<Raw*>(row_of<T>(a.y[w], p.b, p.s, h - (w ? a.heads[0] : 0)));
+          if (l.has0) row[l.v0] = V::pack(reinterpret_cast<float*>(d));
+          if (l.has1) row[l.v1] = V::pack(reinterpret_cast<float*>(d + E / 2));
         }
       }
       p = next;
@@ -668,8 +679,8 @@ bool writes_apart(const Operand& o, const Problem& pr, int w) {
   return (pr.B <= 1 || o.b != 0) && (pr.S <= 1 || o.s != 0) && (pr.H[w] <= 1 || o.h != 0);
 }
 
-bool is_vector_operand(const Operand& o, int64_t E) {
-  return aschost::aligned16(o.p) && o.b % E == 0 && o.s % E == 0 && o.h % E == 0;
+bool is_vector_operand(const Operand& o, int64_t E, int bytes) {
+  return reinterpret_cast<uintptr_t>(o.p) % bytes == 0 && o.b % E == 0 && o.s % E == 0 && o.h % E == 0;
 }
 
 // Checks shared by both directions; *done: there is nothing to compute.
@@ -717,8 +728,8 @@ void fill(RotaryArgs& a, const Problem& pr, const int64_t* pos_strides, const vo
 }
 
 // Lanes per row of the vector kernels, as a power of two; 0 when they do not apply.
-int vector_lanes(const Problem& pr, int interleaved) {
-  const int64_t E = 16 / type_size(pr.dtype);
+int vector_lanes(const Problem& pr, int interleaved, int bytes) {
+  const int64_t E = bytes / type_size(pr.dtype);
   if (pr.D % E != 0 || (!interleaved && (pr.r / 2) % E != 0)) return 0;
   const int64_t n = pr.D / E, hv = pr.r / 2 / E;
   const int64_t units = interleaved ? (n + 1) / 2 : hv + (n - 2 * hv + 1) / 2;
@@ -748,31 +759,53 @@ size_t vector_smem(const RotaryArgs& a) {
   return (a.norm ? 2 * a.D * sizeof(float) : 0) + static_cast<size_t>(kWarps) * (a.r / 2) * sizeof(float2);
 }
 
+// Lanes per row of the vector kernels with vectors of `bytes` for these operands, or 0.
+int lanes_for(const RotaryArgs& a, const Problem& pr, int bytes, bool backward) {
+  const int64_t E = bytes / type_size(pr.dtype);
+  const int lanes = vector_lanes(pr, a.interleaved, bytes);
+  for (int w = 0; w < 2; ++w)
+    if (pr.H[w] > 0 && !(is_vector_operand(a.x[w], E, bytes) && is_vector_operand(a.y[w], E, bytes) &&
+                         (!backward || is_vector_operand(a.dy[w], E, bytes))))
+      return 0;
+  return lanes;
+}
+
+template <typename T, int kBytes>
+void launch_fwd_vectors(RotaryArgs a, int lanes, int sms, cudaStream_t st) {
+  const int64_t tokens = a.tokens;
+  a.log_lanes = log2_of(lanes);
+  a.slices = slices_for(tokens, a.heads[0] > a.heads[1] ? a.heads[0] : a.heads[1], 32 / lanes,
+                        static_cast<int64_t>(kFwdCtas) * kWarps * sms, 2);
+  const int64_t units = tokens * a.slices, most = static_cast<int64_t>(kFwdCtas) * sms;
+  const unsigned grid = static_cast<unsigned>(units < most * kWarps ? (units + kWarps - 1) / kWarps : most);
+  const size_t smem = vector_smem(a);
+  if (a.norm) {
+    if (a.interleaved) rotary_fwd_kernel<T, kBytes, true, true><<<grid, kThreads, smem, st>>>(a);
+    else rotary_fwd_kernel<T, kBytes, true, false><<<grid, kThreads, smem, st>>>(a);
+  } else {
+    if (a.interleaved) rotary_fwd_kernel<T, kBytes, false, true><<<grid, kThreads, smem, st>>>(a);
+    else rotary_fwd_kernel<T, kBytes, false, false><<<grid, kThreads, smem, st>>>(a);
+  }
+}
+
+// 16-byte vectors where sizes, strides and alignment allow; 8-byte ones for 16-bit types that only they divide (halves of
+// 20 elements of a head of 80, say); else element by element, which reads a row twice and costs four to eight times as much.
 template <typename T>
 int32_t launch_fwd(RotaryArgs a, const Problem& pr, cudaStream_t st) {
   int sms = 0;
   int32_t rc = aschost::sm_count(&sms);
   if (rc != ASC_OK) return rc;
-  constexpr int E = Vec<T>::E;
-  const int64_t tokens = a.tokens;
-  int lanes = vector_lanes(pr, a.interleaved);
-  for (int w = 0; w < 2; ++w)
-    if (pr.H[w] > 0 && !(is_vector_operand(a.x[w], E) && is_vector_operand(a.y[w], E))) lanes = 0;
-  if (lanes == 0) {
-    const int64_t grid = tokens < sms * 8ll ? tokens : sms * 8ll;
-    rotary_any_kernel<T, false><<<static_cast<unsigned>(grid), kThreads, a.r / 2 * sizeof(float2), st>>>(a);
+  int lanes = lanes_for(a, pr, 16, false);
+  if (lanes != 0) {
+    launch_fwd_vectors<T, 16>(a, lanes, sms, st);
   } else {
-    a.log_lanes = log2_of(lanes);
-    a.slices = slices_for(tokens, a.heads[0] > a.heads[1] ? a.heads[0] : a.heads[1], 32 / lanes, static_cast<int64_t>(kFwdCtas) * kWarps * sms, 2);
-    const int64_t units = tokens * a.slices, most = static_cast<int64_t>(kFwdCtas) * sms;
-    const unsigned grid = static_cast<unsigned>(units < most * kWarps ? (units + kWarps - 1) / kWarps : most);
-    const size_t smem = vector_smem(a);
-    if (a.norm) {
-      if (a.interleaved) rotary_fwd_kernel<T, true, true><<<grid, kThreads, smem, st>>>(a);
-      else rotary_fwd_kernel<T, true, false><<<grid, kThreads, smem, st>>>(a);
-    } else {
-      if (a.interleaved) rotary_fwd_kernel<T, false, true><<<grid, kThreads, smem, st>>>(a);
-      else rotary_fwd_kernel<T, false, false><<<grid, kThreads, smem, st>>>(a);
+    if constexpr (sizeof(T) == 2) {
+      lanes = lanes_for(a, pr, 8, false);
+      if (lanes != 0) launch_fwd_vectors<T, 8>(a, lanes, sms, st);
+    }
+    if (lanes == 0) {
+      const int64_t tokens = a.tokens, grid = tokens < sms * 8ll ? tokens : sms * 8ll;
+      rotary_any_kernel<T, false><<<static_cast<unsigned>(grid), kThreads, a.r / 2 * sizeof(float2), st>>>(a);
     }
   }
   aschost::count_launch();
@@ -785,12 +818,9 @@ int32_t launch_bwd(RotaryArgs a, const Problem& pr, float* dq_gamma, float* dk_g
   int sms = 0;
   int32_t rc = aschost::sm_count(&sms);
   if (rc != ASC_OK) return rc;
-  constexpr int E = Vec<T>::E;
-  int lanes = vector_lanes(pr, a.interleaved);
-  for (int w = 0; w < 2; ++w)
-    if (pr.H[w] > 0 && !(is_vector_operand(a.x[w], E) && is_vector_operand(a.y[w], E) && is_vector_operand(a.dy[w], E)))
-      lanes = 0;
-  const size_t smem = vector_smem(a) + 2 * E * kThreads * sizeof(float2);
+  int bytes = 16, lanes = lanes_for(a, pr, 16, true);
+  if (lanes == 0 && sizeof(T) == 2) bytes = 8, lanes = lanes_for(a, pr, 8, true);
+  const size_t smem = vector_smem(a) + 2 * (bytes / sizeof(T)) * kThreads * sizeof(float2);
   if (smem > 48 * 1024) lanes = 0;      // 16-bit heads of more than 448: not worth a larger share of the L1 cache
   const int64_t slots = 2ll * sms, H = pr.H[0] + pr.H[1];
   int64_t rows[2];             // rows of partial sums of the gammas, queries' first
@@ -818,8 +848,14 @@ int32_t launch_bwd(RotaryArgs a, const Problem& pr, float* dq_gamma, float* dk_g
     const size_t any_smem = a.r / 2 * sizeof(float2) + static_cast<size_t>(kWarps) * a.D * sizeof(float);
     rotary_any_kernel<T, true><<<static_cast<unsigned>(grid), kThreads, any_smem, st>>>(a);
   } else {
-    if (a.interleaved) rotary_bwd_kernel<T, true><<<static_cast<unsigned>(grid), kThreads, smem, st>>>(a);
-    else rotary_bwd_kernel<T, false><<<static_cast<unsigned>(grid), kThreads, smem, st>>>(a);
+    const unsigned ctas = static_cast<unsigned>(grid);
+    if (bytes == 16) {
+      if (a.interleaved) rotary_bwd_kernel<T, 16, true><<<ctas, kThreads, smem, st>>>(a);
+      else rotary_bwd_kernel<T, 16, false><<<ctas, kThreads, smem, st>>>(a);
+    } else if constexpr (sizeof(T) == 2) {
+      if (a.interleaved) rotary_bwd_kernel<T, 8, true><<<ctas, kThreads, smem, st>>>(a);
+      else rotary_bwd_kernel<T, 8, false><<<ctas, kThreads, smem, st>>>(a);
+    }
   }
   cudaError_t e = cudaGetLastError();
   if (e == cudaSuccess) {

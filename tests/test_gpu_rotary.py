@@ -132,7 +132,7 @@ def test_backward_against_differences():
     assert abs(got - want) <= 1e-6 * ((dx.double() * vx).abs().sum() + (dg.double() * vg).abs().sum())
 
 
-@pytest.mark.parametrize("how", ["misaligned", "odd_pitch", "transposed", "in_place", "expanded"])
+@pytest.mark.parametrize("how", ["misaligned", "eight_bytes", "odd_pitch", "transposed", "in_place", "expanded"])
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 def test_layouts(how, dtype):
     b, s, h, hk, d, r = 2, 21, 4, 2, 64, 64
@@ -142,6 +142,8 @@ def test_layouts(how, dtype):
     out = {}
     if how == "misaligned":
         q, k = (normal((b * s * n * d + 1, ), dtype, n)[1:].view(b, s, n, d) for n in (h, hk))
+    elif how == "eight_bytes":
+        q, k = (normal((b * s * n * d + 4, ), dtype, n)[4:].view(b, s, n, d) for n in (h, hk))
     elif how == "odd_pitch":
         q, k = (normal((b, s, n, d + 3), dtype, n)[..., :d] for n in (h, hk))
         out = {"q_out": torch.empty(b, s, h, d + 1, dtype=dtype, device="cuda")[..., :d]}
